@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define PALIMPSA_ABI_VERSION 13
+#define PALIMPSA_ABI_VERSION 14
 
 /* io dtype of q, k, v, b, o, o_var, do, do_var, dq, dk, dv, db */
 #define PALIMPSA_F32 0
@@ -392,6 +392,122 @@ int palimpsa_layer_prologue_fwd(const palimpsa_layer_prologue *a, void *cuda_str
 int palimpsa_layer_prologue_bwd(const palimpsa_layer_prologue *a, void *cuda_stream);
 int palimpsa_layer_epilogue_fwd(const palimpsa_layer_epilogue *a, void *cuda_stream);
 int palimpsa_layer_epilogue_bwd(const palimpsa_layer_epilogue *a, void *cuda_stream);
+
+/* ---- Operators of the block around the recurrence -------------------------------------------------------
+ * No counterpart in the reference's ops, whose layers take them from flash-linear-attention.  Token rows may lie apart
+ * (`*_stride` elements from one token of the flattened batch to the next, at least the row's length): the layers cut
+ * q, k, v out of one projection.  All other tensors are contiguous.  With cu_seqlens, offsets are read on the device and
+ * clamped to [0, total_tokens]; token rows outside every sequence get zeros in per-token outputs. */
+
+/* Selective state space scan.  Per sequence and head, state h [V,K]:
+ *     dt_t = gt_t, or softplus(gt_t + gt_bias) (PALIMPSA_SSM_SOFTPLUS)      f_t = exp(-g dt_t)
+ *     h_t = f_t h_{t-1} + dt_t v_t k_t^T            o_t = h_t q_t + D v_t
+ * q and k have Hq heads (H % Hq == 0); head h of v reads head h / (H/Hq). */
+#define PALIMPSA_SSM_SOFTPLUS 1u
+typedef struct palimpsa_ssm {
+    size_t struct_size;
+    int32_t io_dtype;               /* of q, k, v, o, d_o, dq, dk, dv                                   */
+    int32_t gt_dtype;               /* of gt, dgt                                                       */
+    uint32_t flags;
+    int32_t num_seqs, H, Hq, K, V;  /* K <= 256, V <= 4096                                              */
+    int64_t seq_len;                /* tokens of each sequence; unused with cu_seqlens                  */
+    int64_t total_tokens;
+    int64_t q_stride, k_stride, v_stride;
+    const void *q, *k;              /* [tokens,Hq,K]                                                    */
+    const void *v;                  /* [tokens,H,V]                                                     */
+    const void *gt;                 /* [tokens,H]                                                       */
+    const float *gt_bias, *g, *D;   /* [H]; gt_bias and D may be NULL                                   */
+    const float *h0;                /* [num_seqs,H,V,K] or NULL: zero                                   */
+    const int32_t *cu_seqlens;      /* [num_seqs+1] or NULL                                             */
+    void *o;                        /* out [tokens,H,V]                                                 */
+    float *h_out;                   /* out [num_seqs,H,V,K] or NULL (step: required, may equal h0)      */
+    void *saved;                    /* forward: written, backward: read; palimpsa_ssm_saved_bytes()     */
+    size_t saved_bytes;
+    /* backward only */
+    const void *d_o;                /* [tokens,H,V]                                                     */
+    const float *dh_out;            /* gradient of h_out, or NULL                                       */
+    void *dq, *dk, *dv;             /* out, contiguous                                                  */
+    void *dgt;                      /* out [tokens,H] gt_dtype                                          */
+    float *dgt_bias, *dg, *dD;      /* out [H]; dgt_bias and dD may be NULL                             */
+    float *dh0;                     /* out [num_seqs,H,V,K] or NULL                                     */
+    void *workspace;                /* >= palimpsa_ssm_workspace_bytes()                                */
+    size_t workspace_bytes;
+} palimpsa_ssm;
+
+/* `training`: a backward will follow (more is kept). 0 if the sizes are not supported. */
+size_t palimpsa_ssm_saved_bytes(const palimpsa_ssm *a, int training);
+size_t palimpsa_ssm_workspace_bytes(const palimpsa_ssm *a);
+/* 1 where the scan runs on the tensor cores (bf16, K and V multiples of 8, K <= 128, aligned rows), else 0. */
+int palimpsa_ssm_plan(const palimpsa_ssm *a);
+int palimpsa_ssm_fwd(const palimpsa_ssm *a, int training, void *cuda_stream);
+int palimpsa_ssm_bwd(const palimpsa_ssm *a, void *cuda_stream);
+/* One token per sequence: total_tokens == num_seqs, cu_seqlens NULL; h_out = the state after it. */
+int palimpsa_ssm_step(const palimpsa_ssm *a, void *cuda_stream);
+
+/* Causal depthwise convolution over the last W inputs of a channel, W = 2, 3 or 4:
+ *     p_t = bias + sum_w weight[d][w] x_{t-(W-1)+w}          y_t = p_t, or p_t sigmoid(p_t) (PALIMPSA_CONV_SILU)
+ * Inputs in front of a sequence are `state` (the W-1 last ones before it, oldest first) or zero. */
+#define PALIMPSA_CONV_SILU 1u
+typedef struct palimpsa_short_conv {
+    size_t struct_size;
+    int32_t io_dtype;
+    int32_t W;
+    uint32_t flags;
+    int32_t num_seqs;
+    int64_t D, seq_len, total_tokens, x_stride;
+    const void *x;                  /* [tokens,D]                                                       */
+    const float *weight, *bias;     /* [D,W]; [D] or NULL                                               */
+    const void *state;              /* [num_seqs,D,W-1] io dtype or NULL                                */
+    const int32_t *cu_seqlens;
+    void *y;                        /* out [tokens,D]                                                   */
+    void *state_out;                /* out [num_seqs,D,W-1] or NULL (step: required, may equal state)   */
+    /* backward only */
+    const void *dy;                 /* [tokens,D]                                                       */
+    const void *dstate_out;         /* gradient of state_out, io dtype, or NULL                         */
+    void *dx;                       /* out [tokens,D]                                                   */
+    float *dweight, *dbias;         /* out [D,W], [D] (dbias may be NULL); summed in a fixed order      */
+    void *dstate;                   /* out [num_seqs,D,W-1] or NULL                                     */
+    void *workspace;
+    size_t workspace_bytes;
+} palimpsa_short_conv;
+size_t palimpsa_short_conv_workspace_bytes(const palimpsa_short_conv *a);
+int palimpsa_short_conv_fwd(const palimpsa_short_conv *a, void *cuda_stream);
+int palimpsa_short_conv_bwd(const palimpsa_short_conv *a, void *cuda_stream);
+int palimpsa_short_conv_step(const palimpsa_short_conv *a, void *cuda_stream);
+
+/* Residual addition and RMS norm over rows of D <= 16384 channels:
+ *     z = x + res (rounded to res's type; z = x without res)      y = z * weight / sqrt(mean(z^2) + eps)
+ * y in the io dtype, or (out_type) in 8 bits with one float32 scale per row or per row and `block` channels
+ * (32, 64, 128 or 256; 0: per row):  s = max(amax |y|, 2^-100) / top (top = 448, 127),  q = y / s to the nearest
+ * value, ties to even -- decided as in 64-bit arithmetic. */
+#define PALIMPSA_NORM_IO 0
+#define PALIMPSA_NORM_E4M3 1
+#define PALIMPSA_NORM_INT8 2
+typedef struct palimpsa_rms_norm {
+    size_t struct_size;
+    int32_t io_dtype;               /* of x, y, dx                                                      */
+    int32_t res_dtype;              /* of res, z, dz: the io dtype or float32; -1: no residual          */
+    int32_t out_type, block;
+    int64_t rows, D;
+    int64_t x_stride;               /* elements from row to row of x                                    */
+    double eps;
+    const void *x, *res;
+    const float *weight;            /* [D]                                                              */
+    void *y;                        /* out [rows,D]                                                     */
+    void *z;                        /* out [rows,D] res dtype; NULL without residual.  backward: input  */
+    float *scale;                   /* out [rows, block ? ceil(D/block) : 1]                            */
+    /* backward only: reads z (x without residual) */
+    const void *dy;                 /* [rows,D] io dtype                                                */
+    const void *dz;                 /* gradient of z, res dtype, or NULL                                */
+    void *dx;                       /* out [rows,D] io dtype                                            */
+    void *dres;                     /* out [rows,D] res dtype; NULL where it equals dx (same type)      */
+    float *dweight;                 /* out [D], summed in a fixed order                                 */
+    void *workspace;
+    size_t workspace_bytes;
+} palimpsa_rms_norm;
+size_t palimpsa_rms_norm_workspace_bytes(const palimpsa_rms_norm *a);
+int palimpsa_rms_norm_fwd(const palimpsa_rms_norm *a, void *cuda_stream);
+int palimpsa_rms_norm_bwd(const palimpsa_rms_norm *a, void *cuda_stream);
 
 #ifdef __cplusplus
 }

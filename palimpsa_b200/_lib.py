@@ -7,7 +7,7 @@ import os
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libpalimpsa_b200.so")
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 F32, BF16, F16 = 0, 1, 2
 FLAG_UNCERTAINTY = 1
 FLAG_EXPLICIT_INIT = 2
@@ -90,6 +90,48 @@ class LayerEpilogue(C.Structure):
     ]
 
 
+SSM_SOFTPLUS, CONV_SILU = 1, 1
+NORM_IO, NORM_E4M3, NORM_INT8 = 0, 1, 2
+
+
+class Ssm(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_size_t), ("io_dtype", C.c_int32), ("gt_dtype", C.c_int32), ("flags", C.c_uint32),
+        ("num_seqs", C.c_int32), ("H", C.c_int32), ("Hq", C.c_int32), ("K", C.c_int32), ("V", C.c_int32),
+        ("seq_len", C.c_int64), ("total_tokens", C.c_int64),
+        ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("gt", C.c_void_p),
+        ("gt_bias", C.c_void_p), ("g", C.c_void_p), ("D", C.c_void_p), ("h0", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("o", C.c_void_p), ("h_out", C.c_void_p), ("saved", C.c_void_p), ("saved_bytes", C.c_size_t),
+        ("d_o", C.c_void_p), ("dh_out", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("dgt", C.c_void_p), ("dgt_bias", C.c_void_p), ("dg", C.c_void_p), ("dD", C.c_void_p), ("dh0", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class ShortConv(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_size_t), ("io_dtype", C.c_int32), ("W", C.c_int32), ("flags", C.c_uint32),
+        ("num_seqs", C.c_int32),
+        ("D", C.c_int64), ("seq_len", C.c_int64), ("total_tokens", C.c_int64), ("x_stride", C.c_int64),
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("state", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("y", C.c_void_p), ("state_out", C.c_void_p),
+        ("dy", C.c_void_p), ("dstate_out", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("dstate", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class RmsNorm(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_size_t), ("io_dtype", C.c_int32), ("res_dtype", C.c_int32), ("out_type", C.c_int32),
+        ("block", C.c_int32),
+        ("rows", C.c_int64), ("D", C.c_int64), ("x_stride", C.c_int64), ("eps", C.c_double),
+        ("x", C.c_void_p), ("res", C.c_void_p), ("weight", C.c_void_p), ("y", C.c_void_p), ("z", C.c_void_p), ("scale", C.c_void_p),
+        ("dy", C.c_void_p), ("dz", C.c_void_p), ("dx", C.c_void_p), ("dres", C.c_void_p), ("dweight", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # every symbol include/palimpsa_b200.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "palimpsa_abi_version": (C.c_int, []),
@@ -133,6 +175,19 @@ SYMBOLS = {
     "palimpsa_layer_prologue_bwd": (C.c_int, [C.POINTER(LayerPrologue), C.c_void_p]),
     "palimpsa_layer_epilogue_fwd": (C.c_int, [C.POINTER(LayerEpilogue), C.c_void_p]),
     "palimpsa_layer_epilogue_bwd": (C.c_int, [C.POINTER(LayerEpilogue), C.c_void_p]),
+    "palimpsa_ssm_saved_bytes": (C.c_size_t, [C.POINTER(Ssm), C.c_int]),
+    "palimpsa_ssm_workspace_bytes": (C.c_size_t, [C.POINTER(Ssm)]),
+    "palimpsa_ssm_plan": (C.c_int, [C.POINTER(Ssm)]),
+    "palimpsa_ssm_fwd": (C.c_int, [C.POINTER(Ssm), C.c_int, C.c_void_p]),
+    "palimpsa_ssm_bwd": (C.c_int, [C.POINTER(Ssm), C.c_void_p]),
+    "palimpsa_ssm_step": (C.c_int, [C.POINTER(Ssm), C.c_void_p]),
+    "palimpsa_short_conv_workspace_bytes": (C.c_size_t, [C.POINTER(ShortConv)]),
+    "palimpsa_short_conv_fwd": (C.c_int, [C.POINTER(ShortConv), C.c_void_p]),
+    "palimpsa_short_conv_bwd": (C.c_int, [C.POINTER(ShortConv), C.c_void_p]),
+    "palimpsa_short_conv_step": (C.c_int, [C.POINTER(ShortConv), C.c_void_p]),
+    "palimpsa_rms_norm_workspace_bytes": (C.c_size_t, [C.POINTER(RmsNorm)]),
+    "palimpsa_rms_norm_fwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p]),
+    "palimpsa_rms_norm_bwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p]),
 }
 
 _lib = None

@@ -20,9 +20,11 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libpalimpsa_b200.so")
 EXT = os.path.join(PKG, "_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
 EXT_STAMP = os.path.join(PKG, "_torch_ops.built_for")      # the torch version EXT was compiled and linked against
-EXT_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
+EXT_UNITS = ("torch_ops", "torch_block")
+EXT_SOURCES = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block.cpp", "torch_common.h")]
 HEADER = os.path.join(ROOT, "include", "palimpsa_b200.h")
-UNITS = ("abi", "fwd", "fwd_tall", "bwd", "decode", "segments", "summary_tc", "carry_tc", "layer", "peer")
+UNITS = ("abi", "fwd", "fwd_tall", "bwd", "decode", "segments", "summary_tc", "carry_tc", "layer", "peer", "conv",
+         "norm", "norm_quant", "ssm", "ssm_tc")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--extended-lambda",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
@@ -35,7 +37,7 @@ def _nvcc() -> str:
 def _sources():
     out = [HEADER]
     for f in sorted(os.listdir(CSRC)):
-        if f.endswith((".cu", ".cuh", ".h")):
+        if f.endswith((".cu", ".cuh", ".h")) and f != "torch_common.h":
             out.append(os.path.join(CSRC, f))
     return out
 
@@ -58,7 +60,7 @@ def _ext_is_for_this_torch() -> bool:
 
 
 def needs_build() -> bool:
-    return _older(LIB, _sources()) or _older(EXT, [HEADER, EXT_SOURCE]) or not _ext_is_for_this_torch()
+    return _older(LIB, _sources()) or _older(EXT, [HEADER, *EXT_SOURCES]) or not _ext_is_for_this_torch()
 
 
 def _run(cmd, what, log=None):
@@ -70,21 +72,22 @@ def _run(cmd, what, log=None):
         raise RuntimeError(f"{what} failed:\n{r.stdout}\n{r.stderr}")
 
 
-def _compile_ext(obj):
-    """The front end's object file: torch's headers, plain host C++."""
+def _compile_ext(unit, obj):
+    """An object file of the front end: torch's headers, plain host C++."""
     from torch.utils import cpp_extension as E
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     inc = [*E.include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_torch_ops",
-          "-DTORCH_API_INCLUDE_EXTENSION_H", *(f"-I{d}" for d in inc), "-c", EXT_SOURCE, "-o", obj], "g++ on torch_ops.cpp")
+          "-DTORCH_API_INCLUDE_EXTENSION_H", *(f"-I{d}" for d in inc), "-c", os.path.join(CSRC, unit + ".cpp"), "-o", obj],
+         f"g++ on {unit}.cpp")
 
 
-def _link_ext(obj):
+def _link_ext(objs):
     import torch
     from torch.utils import cpp_extension as E
     tmp = EXT + ".tmp"
     libs = [f"-L{d}" for d in E.library_paths()]
-    _run(["g++", "-shared", "-o", tmp, obj, f"-L{PKG}", "-l:libpalimpsa_b200.so", *libs, "-ltorch", "-ltorch_cpu",
+    _run(["g++", "-shared", "-o", tmp, *objs, f"-L{PKG}", "-l:libpalimpsa_b200.so", *libs, "-ltorch", "-ltorch_cpu",
           "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN",
           f"-Wl,-rpath,{os.path.join(os.path.dirname(torch.__file__), 'lib')}"], "link of _torch_ops")
     os.replace(tmp, EXT)
@@ -109,17 +112,21 @@ def build(force: bool = False, verbose: bool = False) -> str:
              os.path.join(objdir, u + ".ptxas.log"))
         return obj
 
-    ext_obj = os.path.join(objdir, "torch_ops.o")
-    ext_stale = force or _older(ext_obj, [HEADER, EXT_SOURCE]) or not _ext_is_for_this_torch()
-    with ThreadPoolExecutor(len(UNITS) + 1) as ex:
-        ext_job = ex.submit(_compile_ext, ext_obj) if ext_stale else None
+    def compile_ext_unit(u):
+        obj = os.path.join(objdir, u + ".o")
+        deps = [HEADER, os.path.join(CSRC, u + ".cpp"), os.path.join(CSRC, "torch_common.h")]
+        if force or _older(obj, deps) or not _ext_is_for_this_torch():
+            _compile_ext(u, obj)
+        return obj
+
+    with ThreadPoolExecutor(len(UNITS) + len(EXT_UNITS)) as ex:
+        ext_jobs = ex.map(compile_ext_unit, EXT_UNITS)
         objs = list(ex.map(compile_unit, UNITS))
-        if ext_job:
-            ext_job.result()
+        ext_objs = list(ext_jobs)
     tmp = LIB + ".tmp"
     _run([_nvcc(), "-shared", "-o", tmp, *objs, "-gencode", "arch=compute_100a,code=sm_100a"], "link")
     os.replace(tmp, LIB)
-    _link_ext(ext_obj)
+    _link_ext(ext_objs)
     if verbose:
         print("built", LIB, EXT)
     return LIB

@@ -1,0 +1,440 @@
+// Short causal depthwise convolution with SiLU (sm_100a): what stands in front of q, k and v in the layers.
+//
+//     p_t = bias + sum_j w_j x_{t-(W-1)+j}       y_t = p_t sigmoid(p_t)
+//
+// HBM-bound: x is read and y written once, 2 to 4 FMAs and a sigmoid an element.  A lane owns neighbouring channels (16 bytes
+// in the forward, 4 channels in the backward, whose window, weights and weight gradients fill the registers) and walks a
+// stretch of tokens with the last W inputs in registers, so that a row is read once per stretch and its W-1 rows in front
+// again from L2.  A stretch that holds ends of sequences is walked run by run.
+// Backward: with p recomputed, d_t = dy_t silu'(p_t), dx_t = sum_j w_j d_{t+(W-1)-j}, dw_j = sum_t d_t x_{t-(W-1)+j}: the same
+// walk, W-1 tokens further.  The weight gradients of a CTA's tokens are one row of a workspace, which a second kernel sums in a
+// fixed order (no atomics: results repeat bit by bit).
+#include "block.cuh"
+#include "host.h"
+
+namespace palimpsa {
+
+namespace {
+
+constexpr int WARPS = 4;          // of a CTA: neighbouring stretches of the same channels
+constexpr int FWD_STRETCH = 32;   // tokens a warp walks: 3 rows of 35 are read a second time (L2)
+constexpr int STATE_CHANNELS = 128;
+
+struct ConvArgs {
+    palimpsa_short_conv a;
+    int stretch;       // tokens a warp walks
+    int token_ctas;    // CTAs along the tokens; behind them, one for the states of each sequence
+    bool vec;
+};
+
+// 16-bit types: one exponential and one reciprocal of the special function unit (2^-21 together); float32: full accuracy.
+template <int DT>
+__device__ __forceinline__ float sigmoid_of(float x) {
+    if (DT == PALIMPSA_F32) return __fdiv_rn(1.f, 1.f + expf(-x));
+    return rcp_approx(1.f + __expf(-x));
+}
+
+// Input `t` of the sequence (bos..): a row of x, or what the state holds in front of it.
+template <int DT, int W, int N>
+__device__ __forceinline__ void ld_input(const palimpsa_short_conv& a, int n, long long bos, long long t, long long c, int live,
+                                         bool vec, float (&x)[N]) {
+    if (t >= bos) {
+        ld_n<DT, N>(a.x, t * a.x_stride + c, live, vec, x);
+    } else if (a.state) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            x[i] = i < live ? ld1<DT>(a.state, ((long long)n * a.D + c + i) * (W - 1) + (W - 1 + (t - bos))) : 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = 0.f;
+    }
+}
+
+// The last W-1 inputs of a sequence, one thread per channel.
+template <int DT, int W>
+__device__ __forceinline__ void last_inputs(const palimpsa_short_conv& a, int n, long long c) {
+    long long bos, eos;
+    seq_span(a.cu_seqlens, a.seq_len, a.total_tokens, n, bos, eos);
+    float x[W - 1][1];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) ld_input<DT, W, 1>(a, n, bos, eos - (W - 1) + j, c, 1, false, x[j]);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) st1(a.state_out, ((long long)n * a.D + c) * (W - 1) + j, x[j][0], DT);
+}
+
+template <int DT, int W, bool SILU>
+__global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) {
+    constexpr int N = DT == PALIMPSA_F32 ? 4 : 8;
+    const palimpsa_short_conv& a = g.a;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if ((int)blockIdx.y >= g.token_ctas) {  // final states
+        for (int n = blockIdx.y - g.token_ctas; n < a.num_seqs; n += gridDim.y - g.token_ctas)
+            for (long long c = (long long)blockIdx.x * STATE_CHANNELS + threadIdx.x; c < a.D; c += (long long)gridDim.x * STATE_CHANNELS)
+                last_inputs<DT, W>(a, n, c);
+        return;
+    }
+    const long long c = ((long long)blockIdx.x * 32 + lane) * N;
+    const int live = (int)min((long long)N, a.D - c);  // <= 0: this lane has no channels, but it helps to look up spans
+    float wt[W][N], bias[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        bias[i] = a.bias && i < live ? a.bias[c + i] : 0.f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) wt[j][i] = i < live ? a.weight[(c + i) * W + j] : 0.f;
+    }
+    long long t = ((long long)blockIdx.y * WARPS + w) * g.stretch;
+    const long long end = min(t + g.stretch, (long long)a.total_tokens);
+    while (t < end) {  // a run: the part of one sequence that lies in this stretch
+        const Span s = find_span(a.cu_seqlens, a.num_seqs, a.seq_len, a.total_tokens, t, lane);
+        const long long b = min(end, s.eos);
+        if (live <= 0) {
+            t = b;
+            continue;
+        }
+        if (s.n < 0) {
+            float zero[N] = {};
+            for (; t < b; ++t) st_n<DT, N>(a.y, t * a.D + c, live, g.vec, zero);
+            continue;
+        }
+        float win[W][N];  // win[W-1]: the newest
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j + 1]);
+        constexpr int BATCH = 8;  // rows asked for before the first is used
+        for (; t < b; t += BATCH) {
+            float x[BATCH][N];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                if (t + i < b) ld_n<DT, N>(a.x, (t + i) * a.x_stride + c, live, g.vec, x[i]);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                if (t + i >= b) break;
+                float y[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) win[j][e] = win[j + 1][e];
+                    win[W - 1][e] = x[i][e];
+                    float p = bias[e];
+#pragma unroll
+                    for (int j = 0; j < W; ++j) p = fmaf(wt[j][e], win[j][e], p);
+                    y[e] = SILU ? p * sigmoid_of<DT>(p) : p;
+                }
+                st_n<DT, N>(a.y, (t + i) * a.D + c, live, g.vec, y);
+            }
+        }
+        t = b;
+    }
+}
+
+// d_t of one channel at token t of (n, bos, eos).
+template <int DT, int W, bool SILU>
+__device__ __forceinline__ float d_pre(const palimpsa_short_conv& a, int n, long long bos, long long t, long long c) {
+    float p = a.bias ? a.bias[c] : 0.f, x[1];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        ld_input<DT, W, 1>(a, n, bos, t - (W - 1) + j, c, 1, false, x);
+        p = fmaf(a.weight[c * W + j], x[0], p);
+    }
+    const float dy = ld1<DT>(a.dy, t * a.D + c);
+    if (!SILU) return dy;
+    const float sg = sigmoid_of<DT>(p);
+    return dy * sg * (1.f + p * (1.f - sg));
+}
+
+template <int DT, int W, bool SILU>
+__global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) {
+    constexpr int N = 4;
+    __shared__ float sums[WARPS][W + 1][32 * N];
+    const palimpsa_short_conv& a = g.a;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if ((int)blockIdx.y >= g.token_ctas) {  // gradients of the initial states
+        for (int n = blockIdx.y - g.token_ctas; n < a.num_seqs; n += gridDim.y - g.token_ctas) {
+            long long bos, eos;
+            seq_span(a.cu_seqlens, a.seq_len, a.total_tokens, n, bos, eos);
+            for (long long c = (long long)blockIdx.x * STATE_CHANNELS + threadIdx.x; c < a.D; c += (long long)gridDim.x * STATE_CHANNELS) {
+                float ds[W - 1] = {};
+#pragma unroll
+                for (int t = 0; t < W - 1; ++t) {  // token bos + t reads state i through weight i - t
+                    if (bos + t >= eos) break;
+                    const float d = d_pre<DT, W, SILU>(a, n, bos, bos + t, c);
+#pragma unroll
+                    for (int i = t; i < W - 1; ++i) ds[i] = fmaf(a.weight[c * W + i - t], d, ds[i]);
+                }
+                const long long row = ((long long)n * a.D + c) * (W - 1);
+                if (a.dstate_out) {  // sequences shorter than the state hand some of it on
+#pragma unroll
+                    for (int i = 0; i < W - 1; ++i) {
+                        const long long m = i - (eos - bos);
+                        if (m >= 0) ds[i] += ld1<DT>(a.dstate_out, row + m);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < W - 1; ++i) st1(a.dstate, row + i, ds[i], DT);
+            }
+        }
+        return;
+    }
+    const long long c = ((long long)blockIdx.x * 32 + lane) * N;
+    const int live = (int)min((long long)N, a.D - c);
+    float wt[W][N], bias[N], dw[W][N], db[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        bias[i] = a.bias && i < live ? a.bias[c + i] : 0.f;
+        db[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            wt[j][i] = i < live ? a.weight[(c + i) * W + j] : 0.f;
+            dw[j][i] = 0.f;
+        }
+    }
+    long long t = ((long long)blockIdx.y * WARPS + w) * g.stretch;
+    const long long end = min(t + g.stretch, (long long)a.total_tokens);
+    while (t < end) {
+        const Span s = find_span(a.cu_seqlens, a.num_seqs, a.seq_len, a.total_tokens, t, lane);
+        const long long b = min(end, s.eos);
+        if (live <= 0) {
+            t = b;
+            continue;
+        }
+        if (s.n < 0) {
+            float zero[N] = {};
+            for (; t < b; ++t) st_n<DT, N>(a.dx, t * a.D + c, live, g.vec, zero);
+            continue;
+        }
+        float win[W][N], d[W][N];  // inputs, and d_t of the last W tokens
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j + 1]);
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int e = 0; e < N; ++e) d[j][e] = 0.f;
+        const long long a0 = t, last = b + W - 1;  // tokens t .. last-1, those past eos with d = 0
+        constexpr int BATCH = 4;
+        for (; t < last; t += BATCH) {
+            float x[BATCH][N], dy[BATCH][N];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                if (t + i < last && t + i < s.eos) {
+                    ld_n<DT, N>(a.x, (t + i) * a.x_stride + c, live, g.vec, x[i]);
+                    ld_n<DT, N>(a.dy, (t + i) * a.D + c, live, g.vec, dy[i]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[i][e] = dy[i][e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const long long u = t + i;
+                if (u >= last) break;
+                const bool inside = u < s.eos, own = u < b;
+                float dx[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) win[j][e] = win[j + 1][e], d[j][e] = d[j + 1][e];
+                    win[W - 1][e] = x[i][e];
+                    float dp = dy[i][e];
+                    if (SILU) {
+                        float p = bias[e];
+#pragma unroll
+                        for (int j = 0; j < W; ++j) p = fmaf(wt[j][e], win[j][e], p);
+                        const float sg = sigmoid_of<DT>(p);
+                        dp *= sg * (1.f + p * (1.f - sg));
+                    }
+                    d[W - 1][e] = inside ? dp : 0.f;
+                    if (own) {
+                        db[e] += dp;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) dw[j][e] = fmaf(dp, win[j][e], dw[j][e]);
+                    }
+                    // token u - (W-1): d[j] is that of token u - (W-1) + j, which reads it through weight W-1-j
+                    dx[e] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) dx[e] = fmaf(wt[W - 1 - j][e], d[j][e], dx[e]);
+                }
+                const long long r = u - (W - 1);
+                if (r >= a0) {
+                    if (a.dstate_out && r >= s.eos - (W - 1)) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e)
+                            if (e < live)
+                                dx[e] += ld1<DT>(a.dstate_out, ((long long)s.n * a.D + c + e) * (W - 1) + (r - (s.eos - (W - 1))));
+                    }
+                    st_n<DT, N>(a.dx, r * a.D + c, live, g.vec, dx);
+                }
+            }
+        }
+        t = b;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) sums[w][j][lane * N + e] = dw[j][e];
+        sums[w][W][lane * N + e] = db[e];
+    }
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(a.workspace) + (long long)blockIdx.y * (W + 1) * a.D;
+    for (int i = threadIdx.x; i < (W + 1) * 32 * N; i += 32 * WARPS) {
+        const int j = i / (32 * N), e = i - j * (32 * N);
+        const long long ch = (long long)blockIdx.x * 32 * N + e;
+        if (ch < a.D) {
+            float x = 0.f;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k) x += sums[k][j][e];
+            part[j * a.D + ch] = x;
+        }
+    }
+}
+
+// dweight, dbias from the rows of the workspace: 32 columns x 8 groups of rows a CTA.
+__global__ void __launch_bounds__(256) conv_finish_kernel(const float* part, int parts, int W, long long D, float* dweight, float* dbias) {
+    __shared__ float s[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const long long i = (long long)blockIdx.x * 32 + x, n = (long long)(W + 1) * D;
+    float acc = 0.f;
+    if (i < n)
+        for (int p = y; p < parts; p += 8) acc += part[p * n + i];
+    s[y][x] = acc;
+    __syncthreads();
+    if (y == 0 && i < n) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) acc += s[k][x];
+        const int j = (int)(i / D);
+        const long long d = i - j * D;
+        if (j < W) dweight[d * W + j] = acc;
+        else if (dbias) dbias[d] = acc;
+    }
+}
+
+// One token for each sequence: a thread per channel, states shifted in place.
+template <int DT, int W, bool SILU>
+__global__ void __launch_bounds__(128) conv_step_kernel(const palimpsa_short_conv a) {
+    const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+    if (i >= a.num_seqs * a.D) return;
+    const long long n = i / a.D, c = i - n * a.D;
+    float x[W];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) x[j] = ld1<DT>(a.state, i * (W - 1) + j);
+    x[W - 1] = ld1<DT>(a.x, n * a.x_stride + c);
+    float p = a.bias ? a.bias[c] : 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) p = fmaf(a.weight[c * W + j], x[j], p);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) st1(a.state_out, i * (W - 1) + j, x[j + 1], DT);
+    st1(a.y, i, SILU ? p * sigmoid_of<DT>(p) : p, DT);
+}
+
+int check(const palimpsa_short_conv* a) {
+    if (!a) return PALIMPSA_E_NULL;
+    if (a->struct_size != sizeof(palimpsa_short_conv)) return PALIMPSA_E_VERSION;
+    if (a->num_seqs < 0 || a->D <= 0 || a->seq_len < 0 || a->total_tokens < 0 || a->x_stride < a->D) return PALIMPSA_E_SHAPE;
+    if (!a->cu_seqlens && a->seq_len * a->num_seqs != a->total_tokens) return PALIMPSA_E_SHAPE;
+    if (a->D > (1ll << 30) || a->total_tokens >= (1ll << 31)) return PALIMPSA_E_SHAPE;
+    if (a->W < 2 || a->W > 4) return PALIMPSA_E_DIM;
+    if (a->io_dtype != PALIMPSA_F32 && a->io_dtype != PALIMPSA_BF16 && a->io_dtype != PALIMPSA_F16) return PALIMPSA_E_DTYPE;
+    if (!a->weight || (a->total_tokens > 0 && !a->x)) return PALIMPSA_E_NULL;
+    return PALIMPSA_OK;
+}
+
+template <class F>
+int by_type(const palimpsa_short_conv& a, F&& f) {
+    auto width = [&](auto dt) {
+        auto act = [&](auto w) {
+            return (a.flags & PALIMPSA_CONV_SILU) ? f(dt, w, std::true_type()) : f(dt, w, std::false_type());
+        };
+        return a.W == 2 ? act(std::integral_constant<int, 2>())
+                        : a.W == 3 ? act(std::integral_constant<int, 3>()) : act(std::integral_constant<int, 4>());
+    };
+    return a.io_dtype == PALIMPSA_F32 ? width(std::integral_constant<int, PALIMPSA_F32>())
+           : a.io_dtype == PALIMPSA_BF16 ? width(std::integral_constant<int, PALIMPSA_BF16>())
+                                         : width(std::integral_constant<int, PALIMPSA_F16>());
+}
+int launched() { return cudaGetLastError() == cudaSuccess ? PALIMPSA_OK : PALIMPSA_E_LAUNCH; }
+
+// Tokens a warp of the backward walks: W-1 of them are worked out twice, and every 4 stretches are a row of the workspace, so
+// long ones are cheaper; short ones where the GPU would not be filled (16 warps an SM).
+int bwd_stretch(const palimpsa_short_conv& a) {
+    const long long chunks = (a.D + 127) / 128, per = a.total_tokens * chunks / (B200_SMS * 16);
+    long long n = per >= 64 ? 64 : per <= 8 ? 8 : per & ~3ll;
+    while ((a.total_tokens + n * WARPS - 1) / (n * WARPS) > 49000) n *= 2;  // of the grid's 65535
+    return (int)n;
+}
+long long bwd_parts(const palimpsa_short_conv& a) {
+    const long long per = (long long)bwd_stretch(a) * WARPS;
+    return (a.total_tokens + per - 1) / per;
+}
+unsigned state_ctas(long long seqs) { return (unsigned)(seqs < 16384 ? seqs : 16384); }
+
+}  // namespace
+
+extern "C" {
+
+size_t palimpsa_short_conv_workspace_bytes(const palimpsa_short_conv* a) {
+    if (!a || a->D <= 0 || a->total_tokens < 0 || a->W < 2 || a->W > 4) return 0;
+    return (size_t)(bwd_parts(*a) * (a->W + 1) * a->D) * 4 + 256;
+}
+
+int palimpsa_short_conv_fwd(const palimpsa_short_conv* a, void* stream) {
+    if (int rc = check(a)) return rc;
+    if (a->total_tokens > 0 && !a->y) return PALIMPSA_E_NULL;
+    ConvArgs g{*a, FWD_STRETCH, 0, false};
+    const int n = a->io_dtype == PALIMPSA_F32 ? 4 : 8;
+    g.vec = rows_vec(a->x, a->x_stride, n, a->io_dtype) && rows_vec(a->y, a->D, n, a->io_dtype);
+    const long long chunks = (a->D + 32 * n - 1) / (32 * n);
+    // short batches: shorter stretches, so that more warps share the latency
+    while (g.stretch > 8 && a->total_tokens * chunks < (long long)g.stretch * B200_SMS * 16) g.stretch /= 2;
+    const long long per = (long long)g.stretch * WARPS, ctas = (a->total_tokens + per - 1) / per;
+    const long long states = a->state_out ? state_ctas(a->num_seqs) : 0;
+    if (ctas + states == 0) return PALIMPSA_OK;
+    // the grid's second dimension holds 65535: longer batches take longer stretches
+    while ((a->total_tokens + (long long)g.stretch * WARPS - 1) / ((long long)g.stretch * WARPS) > 49000) g.stretch *= 2;
+    g.token_ctas = (int)((a->total_tokens + (long long)g.stretch * WARPS - 1) / ((long long)g.stretch * WARPS));
+    const dim3 grid((unsigned)chunks, (unsigned)(g.token_ctas + states));
+    return by_type(*a, [&](auto dt, auto w, auto silu) {
+        conv_fwd_kernel<dt.value, w.value, silu.value><<<grid, 32 * WARPS, 0, static_cast<cudaStream_t>(stream)>>>(g);
+        return launched();
+    });
+}
+
+int palimpsa_short_conv_bwd(const palimpsa_short_conv* a, void* stream) {
+    if (int rc = check(a)) return rc;
+    if (!a->dweight || (a->total_tokens > 0 && (!a->dy || !a->dx))) return PALIMPSA_E_NULL;
+    if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 255) ||
+        a->workspace_bytes < palimpsa_short_conv_workspace_bytes(a))
+        return PALIMPSA_E_WORKSPACE;
+    ConvArgs g{*a, bwd_stretch(*a), 0, false};
+    g.vec = rows_vec(a->x, a->x_stride, 4, a->io_dtype) && rows_vec(a->dx, a->D, 4, a->io_dtype) && rows_vec(a->dy, a->D, 4, a->io_dtype);
+    const long long parts = bwd_parts(*a), chunks = (a->D + 127) / 128;
+    const long long states = a->dstate ? state_ctas(a->num_seqs) : 0;
+    g.token_ctas = (int)parts;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (parts + states > 0) {
+        const dim3 grid((unsigned)chunks, (unsigned)(parts + states));
+        const int rc = by_type(*a, [&](auto dt, auto w, auto silu) {
+            conv_bwd_kernel<dt.value, w.value, silu.value><<<grid, 32 * WARPS, 0, st>>>(g);
+            return launched();
+        });
+        if (rc) return rc;
+    }
+    const long long cols = (long long)(a->W + 1) * a->D;
+    conv_finish_kernel<<<(unsigned)((cols + 31) / 32), 256, 0, st>>>(static_cast<const float*>(a->workspace), (int)parts, a->W, a->D,
+                                                                     a->dweight, a->dbias);
+    return launched();
+}
+
+int palimpsa_short_conv_step(const palimpsa_short_conv* a, void* stream) {
+    if (int rc = check(a)) return rc;
+    if (a->cu_seqlens || a->total_tokens != a->num_seqs) return PALIMPSA_E_SHAPE;
+    if (a->num_seqs == 0) return PALIMPSA_OK;
+    if (!a->y || !a->state || !a->state_out) return PALIMPSA_E_NULL;
+    const long long n = a->num_seqs * a->D;
+    if ((n + 127) / 128 > 0x7fffffffll) return PALIMPSA_E_SHAPE;
+    return by_type(*a, [&](auto dt, auto w, auto silu) {
+        conv_step_kernel<dt.value, w.value, silu.value><<<(unsigned)((n + 127) / 128), 128, 0, static_cast<cudaStream_t>(stream)>>>(*a);
+        return launched();
+    });
+}
+
+}  // extern "C"
+
+}  // namespace palimpsa

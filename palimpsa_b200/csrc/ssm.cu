@@ -1,0 +1,809 @@
+// Selective state space scan on the CUDA cores (sm_100a): every type, head size (K <= 256), length and alignment, in float32; the
+// steps that it shares with the tensor-core kernels; and the single-token step.  The formulas are in ssm.cuh.
+//
+// Chunks of 32 tokens: the products inside a chunk cost 32/2 (K + V) FMAs a token and head and the state's 2 K V (K V to make it,
+// K V to read it), and each chunk's state goes through memory three times.
+#include "ssm.cuh"
+
+namespace palimpsa {
+
+namespace {
+
+constexpr int VT = 64;       // rows of V a CTA takes at a time
+constexpr int THREADS = 256;
+
+// ---- chunks of a packed batch -----------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(1024) ssm_plan_kernel(const SsmArgs s) {
+    __shared__ long long warp_sum[32], carry;  // 64 bits: wrong offsets may add up to anything
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, N = s.a.num_seqs;
+    if (tid == 0) carry = 0, s.offset[0] = 0;
+    __syncthreads();
+    for (int n0 = 0; n0 < N; n0 += 1024) {
+        const int n = n0 + tid;
+        long long x = 0;
+        if (n < N) {
+            long long bos, eos;
+            seq_span(s.a.cu_seqlens, 0, s.a.total_tokens, n, bos, eos);
+            x = (eos - bos + s.Q - 1) / s.Q;
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const long long o = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += o;
+        }
+        if (lane == 31) warp_sum[w] = x;
+        __syncthreads();
+        long long before = carry;
+        for (int k = 0; k < w; ++k) before += warp_sum[k];
+        if (n < N) s.offset[n + 1] = (int)min(before + x, (long long)s.chunks);
+        __syncthreads();
+        if (tid == 1023) carry = before + x;
+        __syncthreads();
+    }
+    const int total = N ? s.offset[N] : 0;
+    for (int c = tid; c < s.chunks; c += 1024) {
+        int4 t = make_int4(0, 0, 0, 0);
+        if (c < total) {
+            int lo = 0, hi = N;  // the last n with offset[n] <= c
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (s.offset[mid] <= c) lo = mid;
+                else hi = mid;
+            }
+            long long bos, eos;
+            seq_span(s.a.cu_seqlens, 0, s.a.total_tokens, lo, bos, eos);
+            const long long at = bos + (long long)(c - s.offset[lo]) * s.Q;
+            t = make_int4((int)at, (int)max(0ll, min((long long)s.Q, eos - at)), lo, 0);
+        }
+        s.table[c] = t;
+    }
+}
+
+// Rows of a packed batch that lie in no sequence: zeros.
+struct ZeroRows {
+    void* p[4];
+    long long bytes[4];  // of a row
+    const int* cu;
+    int num_seqs;
+    long long total;
+};
+__global__ void __launch_bounds__(256) ssm_zero_rows_kernel(const ZeroRows z) {
+    const long long first = z.num_seqs ? clamped_offset(z.cu, 0, z.total) : 0;
+    const long long last = z.num_seqs ? clamped_offset(z.cu, z.num_seqs, z.total) : 0;
+    for (int i = 0; i < 4; ++i) {
+        if (!z.p[i]) continue;
+        unsigned short* p = static_cast<unsigned short*>(z.p[i]);
+        const long long row = z.bytes[i] / 2, n0 = first * row, n1 = (z.total - last) * row, step = (long long)gridDim.x * 256;
+        for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n0; e += step) p[e] = 0;
+        for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n1; e += step) p[last * row + e] = 0;
+    }
+}
+
+// ---- dt and L: a warp per chunk and head ------------------------------------------------------------------------------------
+// The sums are taken in 64 bits and kept as two floats: L reaches -14000 (128 tokens of decays that leave nothing), where one
+// float's steps are 1e-3, and e^{L_i-L_j} needs the difference to 1e-7.  A log decay below -110 is e^-110 = 0 all the same.
+template <int PER>  // tokens a lane: Q = 32 PER
+__global__ void __launch_bounds__(256) ssm_prep_kernel(const SsmArgs s) {
+    const palimpsa_ssm& a = s.a;
+    const int lane = threadIdx.x & 31;
+    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (id >= (long long)s.chunks * a.H) return;
+    const int c = (int)(id / a.H), h = (int)(id - (long long)c * a.H);
+    const SsmChunk ch = ssm_chunk(s, c);
+    const bool softplus = (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0;
+    const float bias = a.gt_bias ? a.gt_bias[h] : 0.f;
+    const double g = a.g[h];
+    float dt[PER];
+    double L[PER], sum = 0.;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int t = lane * PER + i;
+        dt[i] = t < ch.len ? ssm_dt(ld_any(a.gt, (ch.tok + t) * a.H + h, a.gt_dtype) + bias, softplus) : 0.f;
+        double lf = t < ch.len ? -g * (double)dt[i] : 0.;
+        if (lf < -110.) lf = -110.;
+        sum += lf;
+        L[i] = sum;
+    }
+    double before = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const double o = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d) before += o;
+    }
+    before -= sum;
+    const long long at = id * s.Q + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const double x = L[i] + before;
+        const float hi = rintf((float)x * 1024.f) * (1.f / 1024.f);
+        s.dt[at + i] = dt[i];
+        s.lh[at + i] = hi;
+        s.ll[at + i] = (float)(x - (double)hi);
+    }
+}
+
+// ---- a chunk's own sum: sum_t w_t a_t b_t^T -----------------------------------------------------------------------------------
+// Forward a = v, b = k, w = e^{L_Q-L_t} dt_t; backward a = do, b = q, w = e^{L_t}.  A thread holds 4 x 4 J of the 64 x K tile.
+template <int DT, int J, bool BACKWARD>
+__global__ void __launch_bounds__(THREADS) ssm_outer_kernel(const SsmArgs s, float* out) {
+    __shared__ __align__(16) float as[SSM_Q][VT];
+    __shared__ __align__(16) float bs[SSM_Q][64 * J];
+    __shared__ float ws[SSM_Q];
+    const palimpsa_ssm& a = s.a;
+    const int tid = threadIdx.x, c = blockIdx.x, h = blockIdx.y, v0 = blockIdx.z * VT;
+    const SsmChunk ch = ssm_chunk(s, c);
+    if (ch.len == 0) return;
+    const int hq = h / (a.H / a.Hq);
+    if (tid < SSM_Q) {
+        const long long at = ((long long)c * a.H + h) * SSM_Q;
+        const float lh = s.lh[at + tid], ll = s.ll[at + tid];
+        ws[tid] = BACKWARD ? expf(lh + ll) : expf((s.lh[at + SSM_Q - 1] - lh) + (s.ll[at + SSM_Q - 1] - ll)) * s.dt[at + tid];
+    }
+    __syncthreads();
+    for (int i = tid; i < SSM_Q * VT; i += THREADS) {
+        const int t = i / VT, v = i % VT;
+        float x = 0.f;
+        if (t < ch.len && v0 + v < a.V)
+            x = ws[t] * (BACKWARD ? ld1<DT>(a.d_o, ((ch.tok + t) * a.H + h) * a.V + v0 + v)
+                                  : ld1<DT>(a.v, (ch.tok + t) * a.v_stride + h * a.V + v0 + v));
+        as[t][v] = x;
+    }
+    for (int i = tid; i < SSM_Q * 64 * J; i += THREADS) {
+        const int t = i / (64 * J), k = i % (64 * J);
+        float x = 0.f;
+        if (t < ch.len && k < a.K)
+            x = BACKWARD ? ld1<DT>(a.q, (ch.tok + t) * a.q_stride + hq * a.K + k) : ld1<DT>(a.k, (ch.tok + t) * a.k_stride + hq * a.K + k);
+        bs[t][k] = x;
+    }
+    __syncthreads();
+    const int ty = tid >> 4, tx = tid & 15;
+    float acc[4][J][4] = {};
+#pragma unroll 4
+    for (int t = 0; t < SSM_Q; ++t) {
+        const float4 x = *reinterpret_cast<const float4*>(&as[t][4 * ty]);
+        const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const float4 y = *reinterpret_cast<const float4*>(&bs[t][64 * j + 4 * tx]);
+            const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[r][j][e] = fmaf(xs[r], ys[e], acc[r][j][e]);
+        }
+    }
+    float* o = out + (((long long)c * a.H + h) * a.V + v0) * a.K;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (v0 + 4 * ty + r < a.V)
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (64 * j + 4 * tx + e < a.K) o[(long long)(4 * ty + r) * a.K + 64 * j + 4 * tx + e] = acc[r][j][e];
+}
+
+// ---- from chunk to chunk: sums become the states in front (gradients behind) of every chunk, in place --------------------------
+template <bool BACKWARD>
+__global__ void __launch_bounds__(256) ssm_scan_kernel(const SsmArgs s) {
+    const palimpsa_ssm& a = s.a;
+    const long long VK = (long long)a.V * a.K;
+    const int n = blockIdx.x / a.H, h = blockIdx.x - n * a.H;
+    const long long e = (long long)blockIdx.y * 256 + threadIdx.x;
+    int first, last;
+    ssm_seq_chunks(s, n, first, last);
+    if (e >= VK) return;
+    const float* start = BACKWARD ? a.dh_out : a.h0;
+    float* end = BACKWARD ? a.dh0 : a.h_out;
+    float* x = BACKWARD ? s.grad : s.state;
+    const long long at = (long long)blockIdx.x * VK + e;
+    float st = start ? start[at] : 0.f;
+    constexpr int AHEAD = 4;
+    for (int c0 = 0; c0 < last - first; c0 += AHEAD) {
+        float y[AHEAD], f[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (c0 + i >= last - first) break;
+            const int c = BACKWARD ? last - 1 - c0 - i : first + c0 + i;
+            const long long ch = (long long)c * a.H + h, l = (ch + 1) * s.Q - 1;
+            y[i] = x[ch * VK + e];
+            f[i] = expf(s.lh[l] + s.ll[l]);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (c0 + i >= last - first) break;
+            const int c = BACKWARD ? last - 1 - c0 - i : first + c0 + i;
+            x[((long long)c * a.H + h) * VK + e] = st;
+            st = fmaf(f[i], st, y[i]);
+        }
+    }
+    if (end) end[at] = st;
+}
+
+// ---- outputs: a CTA per chunk, head and 64 rows of V ---------------------------------------------------------------------------
+__device__ __forceinline__ float decay_between(const float* lh, const float* ll, int i, int j) {
+    return expf((lh[i] - lh[j]) + (ll[i] - ll[j]));
+}
+
+template <int DT>
+__global__ void __launch_bounds__(THREADS) ssm_out_kernel(const SsmArgs s) {
+    extern __shared__ __align__(16) float sm[];
+    const palimpsa_ssm& a = s.a;
+    const int K = a.K, KS = K | 1;  // odd row strides: the rows of a column lie in different banks
+    float* qs = sm;                 // [32][KS]
+    float* ks = qs + SSM_Q * KS;
+    float* vs = ks + SSM_Q * KS;    // [32][65]
+    float* P = vs + SSM_Q * (VT + 1);  // [32][33]
+    float* hs = P + SSM_Q * (SSM_Q + 1);  // [64][33]: 32 columns of the state
+    __shared__ float lh[SSM_Q], ll[SSM_Q], dt[SSM_Q];
+    const int tid = threadIdx.x, c = blockIdx.x, h = blockIdx.y, v0 = blockIdx.z * VT, i = tid >> 3, sub = tid & 7;
+    const SsmChunk ch = ssm_chunk(s, c);
+    if (ch.len == 0) return;
+    const int hq = h / (a.H / a.Hq);
+    if (tid < SSM_Q) {
+        const long long at = ((long long)c * a.H + h) * SSM_Q + tid;
+        lh[tid] = s.lh[at], ll[tid] = s.ll[at], dt[tid] = s.dt[at];
+    }
+    for (int x = tid; x < SSM_Q * K; x += THREADS) {
+        const int t = x / K, k = x - t * K;
+        const bool live = t < ch.len;
+        qs[t * KS + k] = live ? ld1<DT>(a.q, (ch.tok + t) * a.q_stride + hq * K + k) : 0.f;
+        ks[t * KS + k] = live ? ld1<DT>(a.k, (ch.tok + t) * a.k_stride + hq * K + k) : 0.f;
+    }
+    __syncthreads();
+    for (int x = tid; x < SSM_Q * VT; x += THREADS) {  // dt v
+        const int t = x / VT, v = x % VT;
+        vs[t * (VT + 1) + v] = t < ch.len && v0 + v < a.V ? dt[t] * ld1<DT>(a.v, (ch.tok + t) * a.v_stride + h * a.V + v0 + v) : 0.f;
+    }
+    {
+        float S[4] = {};
+        for (int k = 0; k < K; ++k) {
+            const float x = qs[i * KS + k];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[r] = fmaf(x, ks[(4 * sub + r) * KS + k], S[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = 4 * sub + r;
+            P[i * (SSM_Q + 1) + j] = j <= i ? S[r] * decay_between(lh, ll, i, j) : 0.f;
+        }
+    }
+    __syncthreads();
+    float o[8] = {}, inter[8] = {};
+    for (int j = 0; j <= i; ++j) {
+        const float p = P[i * (SSM_Q + 1) + j];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) o[m] = fmaf(p, vs[j * (VT + 1) + sub + 8 * m], o[m]);
+    }
+    const float* hc = s.state + (((long long)c * a.H + h) * a.V + v0) * K;
+    for (int k0 = 0; k0 < K; k0 += 32) {
+        __syncthreads();
+        for (int x = tid; x < VT * 32; x += THREADS) {
+            const int v = x >> 5, k = x & 31;
+            hs[v * 33 + k] = v0 + v < a.V && k0 + k < K ? hc[(long long)v * K + k0 + k] : 0.f;
+        }
+        __syncthreads();
+        const int kn = min(32, K - k0);
+        for (int k = 0; k < kn; ++k) {
+            const float x = qs[i * KS + k0 + k];
+#pragma unroll
+            for (int m = 0; m < 8; ++m) inter[m] = fmaf(x, hs[(sub + 8 * m) * 33 + k], inter[m]);
+        }
+    }
+    if (i < ch.len) {
+        const float e = expf(lh[i] + ll[i]), d = a.D ? a.D[h] : 0.f;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+            const int v = sub + 8 * m;
+            if (v0 + v < a.V) {
+                const float x = a.D ? d * ld1<DT>(a.v, (ch.tok + i) * a.v_stride + h * a.V + v0 + v) : 0.f;
+                st1(a.o, ((ch.tok + i) * a.H + h) * a.V + v0 + v, fmaf(e, inter[m], x + o[m]), DT);
+            }
+        }
+    }
+}
+
+// ---- gradients: a CTA per chunk and head of q and k, over all heads of v that read it ------------------------------------------
+// Thread (i, sub) of 32 x 8 has row i and the columns sub + 8 m of dq and dk.  Sums over heads are taken here, in their order.
+constexpr int VP = 16;  // rows of the state and its gradient in shared memory at a time
+
+size_t grad_smem(int K) {
+    const int KS = K | 1;
+    return sizeof(float) * (size_t)(2 * SSM_Q * KS + 2 * VP * KS + 2 * SSM_Q * (VT + 1) + 4 * SSM_Q * (SSM_Q + 1));
+}
+
+template <int DT, int KM>  // KM: columns of a thread, K <= 8 KM
+__global__ void __launch_bounds__(THREADS) ssm_grad_kernel(const SsmArgs s) {
+    extern __shared__ __align__(16) float sm[];
+    const palimpsa_ssm& a = s.a;
+    constexpr int Q1 = SSM_Q + 1, V1 = VT + 1;
+    const int K = a.K, KS = K | 1;
+    float* qs = sm;                // [32][KS]
+    float* ks = qs + SSM_Q * KS;
+    float* hs = ks + SSM_Q * KS;   // [16][KS]
+    float* gs = hs + VP * KS;
+    float* vs = gs + VP * KS;      // [32][65]
+    float* ds = vs + SSM_Q * V1;
+    float* P = ds + SSM_Q * V1;    // [32][33]: (q_i.k_j) e^{L_i-L_j}
+    float* Mx = P + SSM_Q * Q1;    // M without its diagonal
+    float* PD = Mx + SSM_Q * Q1;   // P_ij (do_i.v_j)
+    float* DS = PD + SSM_Q * Q1;
+    __shared__ float lh[SSM_Q], ll[SSM_Q], dt[SSM_Q], eL[SSM_Q], wq[SSM_Q], As[SSM_Q], Bs[SSM_Q], Zs[SSM_Q], dots[THREADS / 32], dg[SSM_Q];
+    const int tid = threadIdx.x, lane = tid & 31, c = blockIdx.x, hq = blockIdx.y, i = tid >> 3, sub = tid & 7, rep = a.H / a.Hq;
+    const SsmChunk ch = ssm_chunk(s, c);
+    if (ch.len == 0) return;
+    for (int x = tid; x < SSM_Q * K; x += THREADS) {
+        const int t = x / K, k = x - t * K;
+        const bool live = t < ch.len;
+        qs[t * KS + k] = live ? ld1<DT>(a.q, (ch.tok + t) * a.q_stride + hq * K + k) : 0.f;
+        ks[t * KS + k] = live ? ld1<DT>(a.k, (ch.tok + t) * a.k_stride + hq * K + k) : 0.f;
+    }
+    __syncthreads();
+    float S[4] = {}, dSum[4] = {}, dq[KM] = {}, dk[KM] = {};
+    for (int k = 0; k < K; ++k) {
+        const float x = qs[i * KS + k];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[r] = fmaf(x, ks[(4 * sub + r) * KS + k], S[r]);
+    }
+    for (int h = hq * rep; h < (hq + 1) * rep; ++h) {
+        const long long ch_h = (long long)c * a.H + h;
+        __syncthreads();  // the head before is done with everything below
+        if (tid < SSM_Q) {
+            const long long at = ch_h * SSM_Q;
+            lh[tid] = s.lh[at + tid], ll[tid] = s.ll[at + tid], dt[tid] = s.dt[at + tid];
+            eL[tid] = expf(lh[tid] + ll[tid]);
+            wq[tid] = expf((s.lh[at + SSM_Q - 1] - lh[tid]) + (s.ll[at + SSM_Q - 1] - ll[tid]));
+        }
+        __syncthreads();
+        float dec[4], dS[4] = {}, A = 0.f, B = 0.f, dot = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = 4 * sub + r;
+            dec[r] = j <= i ? decay_between(lh, ll, i, j) : 0.f;
+            P[i * Q1 + j] = S[r] * dec[r];
+        }
+        const float D = a.D ? a.D[h] : 0.f;
+        for (int v0 = 0; v0 < a.V; v0 += VT) {
+            __syncthreads();
+            for (int x = tid; x < SSM_Q * VT; x += THREADS) {
+                const int t = x / VT, v = x % VT;
+                const bool live = t < ch.len && v0 + v < a.V;
+                vs[t * V1 + v] = live ? ld1<DT>(a.v, (ch.tok + t) * a.v_stride + h * a.V + v0 + v) : 0.f;
+                ds[t * V1 + v] = live ? ld1<DT>(a.d_o, ((ch.tok + t) * a.H + h) * a.V + v0 + v) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll 4
+            for (int v = 0; v < VT; ++v) {
+                const float x = ds[i * V1 + v];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dS[r] = fmaf(x, vs[(4 * sub + r) * V1 + v], dS[r]);
+            }
+            for (int p0 = 0; p0 < min(VT, a.V - v0); p0 += VP) {
+                const int pn = min(VP, a.V - v0 - p0);
+                if (p0) __syncthreads();
+                const long long at = (ch_h * a.V + v0 + p0) * K;
+                for (int x = tid; x < VP * K; x += THREADS) {
+                    const int v = x / K, k = x - v * K;
+                    const float hv = v < pn ? s.state[at + x] : 0.f, gv = v < pn ? s.grad[at + x] : 0.f;
+                    hs[v * KS + k] = hv, gs[v * KS + k] = gv;
+                    dot = fmaf(hv, gv, dot);
+                }
+                __syncthreads();
+                const float ei = eL[i], wi = wq[i];
+#pragma unroll
+                for (int m = 0; m < KM; ++m) {
+                    const int k = sub + 8 * m;
+                    if (k < K) {
+                        float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+                        for (int v = 0; v < VP; ++v) {
+                            t1 = fmaf(ds[i * V1 + p0 + v], hs[v * KS + k], t1);
+                            t2 = fmaf(vs[i * V1 + p0 + v], gs[v * KS + k], t2);
+                        }
+                        t1 *= ei, t2 *= wi;
+                        dq[m] += t1, dk[m] = fmaf(dt[i], t2, dk[m]);
+                        A = fmaf(qs[i * KS + k], t1, A);
+                        B = fmaf(ks[i * KS + k], t2, B);
+                    }
+                }
+                // dv of row i, columns p0 + sub and p0 + sub + 8
+                float u0 = 0.f, u1 = 0.f;
+                for (int k = 0; k < K; ++k) {
+                    const float x = ks[i * KS + k];
+                    u0 = fmaf(x, gs[sub * KS + k], u0);
+                    u1 = fmaf(x, gs[(sub + 8) * KS + k], u1);
+                }
+                u0 *= wq[i], u1 *= wq[i];
+                for (int r = i; r < SSM_Q; ++r) {
+                    const float p = P[r * Q1 + i];
+                    u0 = fmaf(p, ds[r * V1 + p0 + sub], u0);
+                    u1 = fmaf(p, ds[r * V1 + p0 + sub + 8], u1);
+                }
+                if (i < ch.len) {
+                    const long long row = ((ch.tok + i) * a.H + h) * a.V + v0 + p0;
+                    if (sub < pn) st1(a.dv, row + sub, fmaf(dt[i], u0, D * ds[i * V1 + p0 + sub]), DT);
+                    if (sub + 8 < pn) st1(a.dv, row + sub + 8, fmaf(dt[i], u1, D * ds[i * V1 + p0 + sub + 8]), DT);
+                }
+            }
+        }
+        // what the scalars need
+        float diag = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = 4 * sub + r;
+            const float d = dS[r] * dec[r] * dt[j];
+            dSum[r] += d;
+            Mx[i * Q1 + j] = j < i ? d * S[r] : 0.f;
+            PD[i * Q1 + j] = S[r] * dec[r] * dS[r];
+            if (j == i) diag = dS[r];
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) {
+            A += __shfl_xor_sync(0xffffffffu, A, o);
+            B += __shfl_xor_sync(0xffffffffu, B, o);
+            diag += __shfl_xor_sync(0xffffffffu, diag, o);
+        }
+        dot = warp_add(dot);
+        if (sub == 0) As[i] = A, Bs[i] = B, dg[i] = diag;
+        if (lane == 0) dots[tid >> 5] = dot;
+        __syncthreads();
+        {   // sum_{i>=t>j} M_ij term by term: as a difference of sums it would not vanish where the decays do
+            float z = 0.f;
+            for (int r = i + sub; r < SSM_Q; r += 8)
+                for (int j = 0; j < i; ++j) z += Mx[r * Q1 + j];
+#pragma unroll
+            for (int o = 1; o < 8; o *= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
+            if (sub == 0) Zs[i] = z;
+        }
+        __syncthreads();
+        if (tid < 32) {
+            const int t = lane;
+            double hG = 0.;
+#pragma unroll
+            for (int k = 0; k < THREADS / 32; ++k) hG += dots[k];
+            float direct = 0.f;
+            for (int k = t; k < SSM_Q; ++k) direct += PD[k * Q1 + t];
+            const double own = (double)dt[t] * Bs[t];
+            double suf = As[t], pre = own;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const double x = __shfl_down_sync(0xffffffffu, suf, d), y = __shfl_up_sync(0xffffffffu, pre, d);
+                if (t + d < 32) suf += x;
+                if (t >= d) pre += y;
+            }
+            const double in = __shfl_up_sync(0xffffffffu, pre, 1);  // of the tokens before: pre - own would leave a remainder
+            const double dlf = (double)Zs[t] + suf + (t ? in : 0.) + (double)eL[SSM_Q - 1] * hG;
+            float ddt = (float)((double)direct + (double)Bs[t] - (double)a.g[h] * dlf);
+            double pg = 0., pb = 0., pd = 0.;
+            if (t < ch.len) {
+                const long long at = (ch.tok + t) * a.H + h;
+                const float u = ld_any(a.gt, at, a.gt_dtype) + (a.gt_bias ? a.gt_bias[h] : 0.f);
+                ddt *= ssm_ddt(u, (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0);
+                st1(a.dgt, at, ddt, a.gt_dtype);
+                pg = -(double)dt[t] * dlf, pb = ddt, pd = dg[t];
+            }
+            pg = warp_add(pg), pb = warp_add(pb), pd = warp_add(pd);
+            if (lane == 0) {
+                const long long n = (long long)s.chunks * a.H;
+                s.part[ch_h] = (float)pg, s.part[n + ch_h] = (float)pb, s.part[2 * n + ch_h] = (float)pd;
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) DS[i * Q1 + 4 * sub + r] = dSum[r];
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < KM; ++m) {
+        const int k = sub + 8 * m;
+        if (k < K && i < ch.len) {
+            float x = dq[m], y = dk[m];
+            for (int j = 0; j <= i; ++j) x = fmaf(DS[i * Q1 + j], ks[j * KS + k], x);
+            for (int r = i; r < SSM_Q; ++r) y = fmaf(DS[r * Q1 + i], qs[r * KS + k], y);
+            const long long at = ((ch.tok + i) * a.Hq + hq) * K + k;
+            st1(a.dq, at, x, DT);
+            st1(a.dk, at, y, DT);
+        }
+    }
+}
+
+// dg, dgt_bias, dD of a head: the chunks' shares in a fixed order, in 64 bits.
+__global__ void __launch_bounds__(256) ssm_finish_kernel(const SsmArgs s) {
+    __shared__ double x[3][8];
+    const palimpsa_ssm& a = s.a;
+    const int h = blockIdx.x, tid = threadIdx.x;
+    const long long n = (long long)s.chunks * a.H;
+    double sum[3] = {0., 0., 0.};
+    for (int c = tid; c < s.chunks; c += 256) {
+        if (ssm_chunk(s, c).len == 0) continue;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) sum[k] += s.part[k * n + (long long)c * a.H + h];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        sum[k] = warp_add(sum[k]);
+        if ((tid & 31) == 0) x[k][tid >> 5] = sum[k];
+    }
+    __syncthreads();
+    if (tid < 3) {
+        double t = 0.;
+        for (int w = 0; w < 8; ++w) t += x[tid][w];
+        float* out = tid == 0 ? a.dg : tid == 1 ? a.dgt_bias : a.dD;
+        if (out) out[h] = (float)t;
+    }
+}
+
+// ---- one token for each sequence -----------------------------------------------------------------------------------------------
+// HBM-bound: the state is read and written once.  LANES lanes share a row of the state, 4 neighbouring columns each (NK times);
+// the loads of ROWS rows are issued before the first is used.
+template <int DT, int LANES, int NK, bool VEC>
+__global__ void __launch_bounds__(128) ssm_step_kernel(const SsmArgs s) {
+    constexpr int ROWS = NK == 1 ? 8 : 4, GROUPS = 128 / LANES;
+    const palimpsa_ssm& a = s.a;
+    const int tid = threadIdx.x, sub = tid % LANES, grp = tid / LANES;
+    const int n = blockIdx.x / a.H, h = blockIdx.x - n * a.H, hq = h / (a.H / a.Hq);
+    const long long nh = blockIdx.x;
+    const int v0 = (blockIdx.y * GROUPS + grp) * ROWS;
+    float* out = a.h_out + nh * a.V * a.K;
+    const float* in = a.h0 + nh * a.V * a.K;
+    float st[ROWS][NK][4];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int m = 0; m < NK; ++m) {
+            const int c = 4 * (sub + m * LANES);
+            if (v0 + r < a.V) ld_n<PALIMPSA_F32, 4>(in, (long long)(v0 + r) * a.K + c, a.K - c, VEC && c < a.K, st[r][m]);
+        }
+    float q[NK][4], k[NK][4];
+#pragma unroll
+    for (int m = 0; m < NK; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = 4 * (sub + m * LANES) + e;
+            q[m][e] = c < a.K ? ld1<DT>(a.q, n * a.q_stride + hq * a.K + c) : 0.f;
+            k[m][e] = c < a.K ? ld1<DT>(a.k, n * a.k_stride + hq * a.K + c) : 0.f;
+        }
+    const float dt = ssm_dt(ld_any(a.gt, nh, a.gt_dtype) + (a.gt_bias ? a.gt_bias[h] : 0.f), (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0);
+    const float f = expf(-a.g[h] * dt), D = a.D ? a.D[h] : 0.f;
+    float o[ROWS], v[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        o[r] = 0.f;
+        v[r] = v0 + r < a.V ? ld1<DT>(a.v, n * a.v_stride + h * a.V + v0 + r) : 0.f;
+        const float x = dt * v[r];
+        if (v0 + r < a.V) {
+#pragma unroll
+            for (int m = 0; m < NK; ++m) {
+                const int c = 4 * (sub + m * LANES);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    st[r][m][e] = fmaf(f, st[r][m][e], x * k[m][e]);
+                    if (VEC || c + e < a.K) o[r] = fmaf(st[r][m][e], q[m][e], o[r]);
+                }
+                if (c < a.K) st_n<PALIMPSA_F32, 4>(out, (long long)(v0 + r) * a.K + c, a.K - c, VEC, st[r][m]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+        for (int off = LANES / 2; off >= 1; off >>= 1) o[r] += __shfl_xor_sync(0xffffffffu, o[r], off);
+        if (sub == 0 && v0 + r < a.V) st1(a.o, nh * a.V + v0 + r, fmaf(D, v[r], o[r]), DT);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+int check(const palimpsa_ssm* a) {
+    if (!a) return PALIMPSA_E_NULL;
+    if (a->struct_size != sizeof(palimpsa_ssm)) return PALIMPSA_E_VERSION;
+    if (a->num_seqs < 0 || a->H <= 0 || a->Hq <= 0 || a->H % a->Hq || a->K <= 0 || a->V <= 0 || a->seq_len < 0 || a->total_tokens < 0)
+        return PALIMPSA_E_SHAPE;
+    if (!a->cu_seqlens && a->seq_len * a->num_seqs != a->total_tokens) return PALIMPSA_E_SHAPE;
+    if (a->K > PALIMPSA_MAX_K || a->V > 4096) return PALIMPSA_E_DIM;
+    if (a->H > 65535 || a->num_seqs * (long long)a->H >= (1ll << 31)) return PALIMPSA_E_SHAPE;
+    for (int d : {a->io_dtype, a->gt_dtype})
+        if (d != PALIMPSA_F32 && d != PALIMPSA_BF16 && d != PALIMPSA_F16) return PALIMPSA_E_DTYPE;
+    if (a->q_stride < (int64_t)a->Hq * a->K || a->k_stride < (int64_t)a->Hq * a->K || a->v_stride < (int64_t)a->H * a->V)
+        return PALIMPSA_E_SHAPE;
+    if (a->total_tokens * a->H >= (1ll << 31)) return PALIMPSA_E_SHAPE;
+    if (!a->g || (a->total_tokens > 0 && (!a->q || !a->k || !a->v || !a->gt))) return PALIMPSA_E_NULL;
+    return PALIMPSA_OK;
+}
+long long chunk_room(const palimpsa_ssm& a, int Q) {
+    return a.cu_seqlens ? a.total_tokens / Q + a.num_seqs : a.num_seqs * ((a.seq_len + Q - 1) / Q);
+}
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct Layout {
+    bool tc;
+    int Q;
+    long long chunks;
+    size_t table, offset, dt, lh, ll, state, saved;  // of `saved`
+    size_t grad, part, workspace;                    // of the workspace
+};
+Layout layout(const palimpsa_ssm& a, bool training) {
+    Layout l{};
+    l.tc = ssm_tc_supported(a);
+    l.Q = l.tc ? SSM_TC_Q : SSM_Q;
+    l.chunks = chunk_room(a, l.Q);
+    const size_t scalars = up256((size_t)l.chunks * a.H * l.Q * 4), states = up256((size_t)l.chunks * a.H * a.V * a.K * 4);
+    size_t at = 0;
+    auto take = [&at](size_t n) {
+        const size_t r = at;
+        at += up256(n);
+        return r;
+    };
+    l.table = take(a.cu_seqlens ? (size_t)l.chunks * 16 : 0);
+    l.offset = take(a.cu_seqlens ? ((size_t)a.num_seqs + 1) * 4 : 0);
+    l.dt = take(scalars), l.lh = take(scalars), l.ll = take(scalars);
+    l.state = take(l.tc ? ssm_tc_state_bytes(a, l.chunks, training) : states);
+    l.saved = at + 256;
+    at = 0;
+    l.grad = take(l.tc ? ssm_tc_workspace_bytes(a, l.chunks) : states);
+    l.part = take((size_t)l.chunks * a.H * 12);
+    l.workspace = at + 256;
+    return l;
+}
+SsmArgs args_of(const palimpsa_ssm& a, const Layout& l) {
+    SsmArgs s{};
+    s.a = a;
+    s.Q = l.Q, s.chunks = (int)l.chunks, s.per_seq = (int)((a.seq_len + l.Q - 1) / l.Q);
+    char* p = static_cast<char*>(a.saved);
+    if (a.cu_seqlens) s.table = reinterpret_cast<int4*>(p + l.table), s.offset = reinterpret_cast<int*>(p + l.offset);
+    s.dt = reinterpret_cast<float*>(p + l.dt), s.lh = reinterpret_cast<float*>(p + l.lh), s.ll = reinterpret_cast<float*>(p + l.ll);
+    s.state = reinterpret_cast<float*>(p + l.state);
+    if (a.workspace) {
+        char* w = static_cast<char*>(a.workspace);
+        s.grad = reinterpret_cast<float*>(w + l.grad), s.part = reinterpret_cast<float*>(w + l.part);
+    }
+    return s;
+}
+bool misaligned256(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 255) != 0; }
+int launched() { return cudaGetLastError() == cudaSuccess ? PALIMPSA_OK : PALIMPSA_E_LAUNCH; }
+
+template <class F>
+int by_type(int dt, F&& f) {
+    return dt == PALIMPSA_F32 ? f(std::integral_constant<int, PALIMPSA_F32>())
+           : dt == PALIMPSA_BF16 ? f(std::integral_constant<int, PALIMPSA_BF16>())
+                                 : f(std::integral_constant<int, PALIMPSA_F16>());
+}
+
+template <bool BACKWARD>
+int launch_sums(const SsmArgs& s, cudaStream_t st) {
+    const palimpsa_ssm& a = s.a;
+    float* out = BACKWARD ? s.grad : s.state;
+    int rc = PALIMPSA_OK;
+    if (s.chunks > 0) {
+        const dim3 grid(s.chunks, a.H, (a.V + VT - 1) / VT);
+        rc = by_type(a.io_dtype, [&](auto dt) {
+            if (a.K <= 64) ssm_outer_kernel<dt.value, 1, BACKWARD><<<grid, THREADS, 0, st>>>(s, out);
+            else if (a.K <= 128) ssm_outer_kernel<dt.value, 2, BACKWARD><<<grid, THREADS, 0, st>>>(s, out);
+            else ssm_outer_kernel<dt.value, 4, BACKWARD><<<grid, THREADS, 0, st>>>(s, out);
+            return launched();
+        });
+        if (rc) return rc;
+    }
+    const long long VK = (long long)a.V * a.K, rows = (long long)a.num_seqs * a.H;
+    if (rows > 0) ssm_scan_kernel<BACKWARD><<<dim3((unsigned)rows, (unsigned)((VK + 255) / 256)), 256, 0, st>>>(s);
+    return launched();
+}
+
+}  // namespace
+
+// dt, L and, in a packed batch, the chunks and the rows outside: what a forward begins with.
+static int launch_prep(const SsmArgs& s, cudaStream_t st) {
+    if (s.a.cu_seqlens && s.chunks + s.a.num_seqs > 0) ssm_plan_kernel<<<1, 1024, 0, st>>>(s);
+    const long long warps = (long long)s.chunks * s.a.H;
+    if (warps > 0) {
+        const unsigned ctas = (unsigned)((warps + 7) / 8);
+        if (s.Q == 32) ssm_prep_kernel<1><<<ctas, 256, 0, st>>>(s);
+        else ssm_prep_kernel<SSM_TC_Q / 32><<<ctas, 256, 0, st>>>(s);
+    }
+    return launched();
+}
+
+extern "C" {
+
+size_t palimpsa_ssm_saved_bytes(const palimpsa_ssm* a, int training) {
+    return a && (check(a) == PALIMPSA_OK || check(a) == PALIMPSA_E_NULL) ? layout(*a, training != 0).saved : 0;
+}
+size_t palimpsa_ssm_workspace_bytes(const palimpsa_ssm* a) {
+    return a && (check(a) == PALIMPSA_OK || check(a) == PALIMPSA_E_NULL) ? layout(*a, true).workspace : 0;
+}
+int palimpsa_ssm_plan(const palimpsa_ssm* a) { return a && ssm_tc_supported(*a) ? 1 : 0; }
+
+int palimpsa_ssm_fwd(const palimpsa_ssm* a, int training, void* stream) {
+    if (int rc = check(a)) return rc;
+    if (a->total_tokens > 0 && !a->o) return PALIMPSA_E_NULL;
+    const Layout l = layout(*a, training != 0);
+    if (!a->saved || misaligned256(a->saved) || a->saved_bytes < l.saved) return PALIMPSA_E_WORKSPACE;
+    if (l.chunks >= (1ll << 31)) return PALIMPSA_E_SHAPE;
+    if (a->num_seqs == 0 && a->total_tokens == 0) return PALIMPSA_OK;
+    const SsmArgs s = args_of(*a, l);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (int rc = launch_prep(s, st)) return rc;
+    if (a->cu_seqlens && a->total_tokens > 0) {
+        const ZeroRows z{{a->o}, {(long long)a->H * a->V * dtype_size(a->io_dtype)}, a->cu_seqlens, a->num_seqs, a->total_tokens};
+        ssm_zero_rows_kernel<<<64, 256, 0, st>>>(z);
+    }
+    if (l.tc) return ssm_tc_fwd(s, training != 0, st);
+    if (int rc = launch_sums<false>(s, st)) return rc;
+    if (s.chunks == 0) return PALIMPSA_OK;
+    const int KS = a->K | 1;
+    const size_t smem = sizeof(float) * (size_t)(2 * SSM_Q * KS + SSM_Q * (VT + 1) + SSM_Q * (SSM_Q + 1) + VT * 33);
+    return by_type(a->io_dtype, [&](auto dt) {
+        if (!allow_smem<ssm_out_kernel<dt.value>>((int)smem)) return (int)PALIMPSA_E_LAUNCH;
+        ssm_out_kernel<dt.value><<<dim3(s.chunks, a->H, (a->V + VT - 1) / VT), THREADS, smem, st>>>(s);
+        return launched();
+    });
+}
+
+int palimpsa_ssm_bwd(const palimpsa_ssm* a, void* stream) {
+    if (int rc = check(a)) return rc;
+    if (!a->dg || (a->total_tokens > 0 && (!a->d_o || !a->dq || !a->dk || !a->dv || !a->dgt))) return PALIMPSA_E_NULL;
+    const Layout l = layout(*a, true);
+    if (!a->saved || misaligned256(a->saved) || a->saved_bytes < l.saved) return PALIMPSA_E_WORKSPACE;
+    if (!a->workspace || misaligned256(a->workspace) || a->workspace_bytes < l.workspace) return PALIMPSA_E_WORKSPACE;
+    if (l.chunks >= (1ll << 31)) return PALIMPSA_E_SHAPE;
+    const SsmArgs s = args_of(*a, l);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->cu_seqlens && a->total_tokens > 0) {
+        const long long io = dtype_size(a->io_dtype), qk = (long long)a->Hq * a->K * io;
+        const ZeroRows z{{a->dq, a->dk, a->dv, a->dgt}, {qk, qk, (long long)a->H * a->V * io, (long long)a->H * dtype_size(a->gt_dtype)},
+                         a->cu_seqlens, a->num_seqs, a->total_tokens};
+        ssm_zero_rows_kernel<<<64, 256, 0, st>>>(z);
+    }
+    if (l.tc) {
+        if (int rc = ssm_tc_bwd(s, st)) return rc;
+    } else {
+        if (int rc = launch_sums<true>(s, st)) return rc;
+        if (s.chunks > 0) {
+            const size_t smem = grad_smem(a->K);
+            const int rc = by_type(a->io_dtype, [&](auto dt) {
+                auto go = [&](auto km) {
+                    if (!allow_smem<ssm_grad_kernel<dt.value, km.value>>((int)smem)) return (int)PALIMPSA_E_LAUNCH;
+                    ssm_grad_kernel<dt.value, km.value><<<dim3(s.chunks, a->Hq), THREADS, smem, st>>>(s);
+                    return launched();
+                };
+                if (a->K <= 32) return go(std::integral_constant<int, 4>());
+                if (a->K <= 64) return go(std::integral_constant<int, 8>());
+                if (a->K <= 128) return go(std::integral_constant<int, 16>());
+                return go(std::integral_constant<int, 32>());
+            });
+            if (rc) return rc;
+        }
+    }
+    ssm_finish_kernel<<<a->H, 256, 0, st>>>(s);
+    return launched();
+}
+
+int palimpsa_ssm_step(const palimpsa_ssm* a, void* stream) {
+    if (int rc = check(a)) return rc;
+    if (a->cu_seqlens || a->total_tokens != a->num_seqs) return PALIMPSA_E_SHAPE;
+    if (a->num_seqs == 0) return PALIMPSA_OK;
+    if (!a->o || !a->h0 || !a->h_out) return PALIMPSA_E_NULL;
+    SsmArgs s{};
+    s.a = *a;
+    const bool vec = a->K % 4 == 0 && ((reinterpret_cast<uintptr_t>(a->h0) | reinterpret_cast<uintptr_t>(a->h_out)) & 15) == 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long rows = (long long)a->num_seqs * a->H;
+    if (rows >= (1ll << 31)) return PALIMPSA_E_SHAPE;
+    return by_type(a->io_dtype, [&](auto dt) {
+        auto go = [&](auto lanes, auto nk) {
+            const int per = 128 / lanes.value * (nk.value == 1 ? 8 : 4);
+            const dim3 grid((unsigned)rows, (a->V + per - 1) / per);
+            if (vec) ssm_step_kernel<dt.value, lanes.value, nk.value, true><<<grid, 128, 0, st>>>(s);
+            else ssm_step_kernel<dt.value, lanes.value, nk.value, false><<<grid, 128, 0, st>>>(s);
+            return launched();
+        };
+        using std::integral_constant;
+        if (a->K <= 16) return go(integral_constant<int, 4>(), integral_constant<int, 1>());
+        if (a->K <= 32) return go(integral_constant<int, 8>(), integral_constant<int, 1>());
+        if (a->K <= 64) return go(integral_constant<int, 16>(), integral_constant<int, 1>());
+        if (a->K <= 128) return go(integral_constant<int, 32>(), integral_constant<int, 1>());
+        return go(integral_constant<int, 32>(), integral_constant<int, 2>());
+    });
+}
+
+}  // extern "C"
+
+}  // namespace palimpsa

@@ -1,0 +1,78 @@
+// Selective state space scan: layout of its buffers and what its kernels share (ssm.cu, ssm_tc.cu).
+//
+//     h_t = f_t h_{t-1} + dt_t v_t k_t^T      o_t = h_t q_t + D v_t      f_t = exp(-g dt_t)
+//
+// A sequence is cut into chunks of Q tokens.  With L_i the sum of log f from the chunk's start to token i, h the state in front of
+// the chunk and G the gradient of the state behind it:
+//     o_i   = sum_{j<=i} (q_i.k_j) e^{L_i-L_j} dt_j v_j + e^{L_i} h q_i + D v_i       h' = e^{L_Q} h + sum_j w_j dt_j v_j k_j^T
+//     G'    = e^{L_Q} G + sum_i e^{L_i} do_i q_i^T                                    w_j = e^{L_Q-L_j}
+//     dv_j  = dt_j (sum_{i>=j} (q_i.k_j) e^{L_i-L_j} do_i + w_j G k_j) + D do_j
+//     dq_i  = sum_{j<=i} dS_ij k_j + e^{L_i} h^T do_i        dS_ij = (do_i.v_j) e^{L_i-L_j} dt_j
+//     dk_j  = sum_{i>=j} dS_ij q_i + w_j dt_j G^T v_j
+// and, with M_ij = dS_ij (q_i.k_j), the gradient of log f_t is what flows across the border in front of t:
+//     sum_{i>=t>j} M_ij + sum_{i>=t} e^{L_i} do_i.(h q_i) + sum_{j<t} w_j dt_j v_j.(G k_j) + e^{L_Q} <h, G>
+// All exponents are differences L_i - L_j <= 0, so nothing overflows and no decay is divided by.
+//
+// Steps: prep (dt and L) -> the chunks' own sums (states: w dt v k^T; gradients: e^L do q^T) and their scan from chunk to chunk ->
+// all chunks side by side.  Kernels on CUDA cores (any type and size, Q = 32, float32 throughout) in ssm.cu, on the tensor cores
+// (bf16, Q = 128) in ssm_tc.cu.
+#pragma once
+
+#include "block.cuh"
+#include "host.h"
+
+namespace palimpsa {
+
+constexpr int SSM_Q = 32;      // tokens of a chunk on the CUDA cores
+constexpr int SSM_TC_Q = 128;  // and on the tensor cores
+
+struct SsmArgs {
+    palimpsa_ssm a;
+    int Q, chunks, per_seq;  // chunks: room for them; per_seq: of a sequence where all are equally long
+    int4* table;             // [chunks] {first token, tokens, sequence, -} of a packed batch
+    int* offset;             // [num_seqs+1] first chunk of a sequence of a packed batch
+    float *dt, *lh, *ll;     // [chunks][H][Q]: dt, and L as lh + ll, lh a multiple of 2^-10: lh_i - lh_j is exact
+    float* state;            // [chunks][H][V][K]: the state in front of every chunk
+    float* grad;             // [chunks][H][V][K]: backward, the gradient of the state behind every chunk
+    float* part;             // [3][chunks][H]: shares of dg, dgt_bias, dD
+};
+
+struct SsmChunk {
+    long long tok;  // first token
+    int len, n;     // len 0: no chunk
+};
+__device__ __forceinline__ SsmChunk ssm_chunk(const SsmArgs& s, int c) {
+    SsmChunk r;
+    if (s.table) {
+        const int4 t = s.table[c];
+        r.tok = t.x, r.len = t.y, r.n = t.z;
+    } else {
+        r.n = c / s.per_seq;
+        const long long at = (long long)(c - r.n * s.per_seq) * s.Q, left = s.a.seq_len - at;
+        r.tok = r.n * s.a.seq_len + at;
+        r.len = left < s.Q ? (int)left : s.Q;
+    }
+    return r;
+}
+__device__ __forceinline__ void ssm_seq_chunks(const SsmArgs& s, int n, int& first, int& last) {
+    if (s.table) {
+        first = min(s.offset[n], s.chunks), last = min(s.offset[n + 1], s.chunks);
+    } else {
+        first = n * s.per_seq, last = first + s.per_seq;
+    }
+}
+__device__ __forceinline__ float ld_any(const void* p, long long i, int dt) {
+    return dt == PALIMPSA_F32 ? ld1<PALIMPSA_F32>(p, i) : dt == PALIMPSA_BF16 ? ld1<PALIMPSA_BF16>(p, i) : ld1<PALIMPSA_F16>(p, i);
+}
+// torch's softplus (threshold 20) and its derivative
+__device__ __forceinline__ float ssm_dt(float u, bool softplus) { return !softplus || u > 20.f ? u : log1pf(expf(u)); }
+__device__ __forceinline__ float ssm_ddt(float u, bool softplus) { return !softplus || u > 20.f ? 1.f : __fdiv_rn(1.f, 1.f + expf(-u)); }
+
+// Kernels on the tensor cores (ssm_tc.cu).
+bool ssm_tc_supported(const palimpsa_ssm& a);
+size_t ssm_tc_state_bytes(const palimpsa_ssm& a, long long chunks, bool training);
+size_t ssm_tc_workspace_bytes(const palimpsa_ssm& a, long long chunks);
+int ssm_tc_fwd(const SsmArgs& s, bool training, cudaStream_t stream);
+int ssm_tc_bwd(const SsmArgs& s, cudaStream_t stream);
+
+}  // namespace palimpsa

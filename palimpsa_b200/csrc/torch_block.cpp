@@ -1,0 +1,495 @@
+// Torch front end of the operators around the recurrence: the state space scan, the short convolution, the residual norm.
+// Checks, allocation, autograd nodes and the calls into the C ABI; palimpsa_b200/layers.py and ops/ssm.py document them.
+#include "torch_common.h"
+
+namespace palimpsa_torch {
+
+namespace {
+
+// These calls run eagerly: under a tracer, a transform or a mode there is no data to point at.
+void require_plain(const char* name, std::initializer_list<const Tensor*> ts) {
+    require_cuda(ts);
+    TORCH_CHECK(plain(ts), name, " takes dense CUDA tensors and runs eagerly: it cannot be traced, transformed or run under a mode");
+}
+void require_same_device(const char* name, const Tensor& first, std::initializer_list<std::pair<const char*, const Tensor*>> ts) {
+    for (auto& [n, t] : ts)
+        TORCH_CHECK_VALUE(!t->defined() || t->device() == first.device(), name, ": ", n, " is on ", t->device(), ", not on ", first.device());
+}
+// Gradients of these nodes are made by kernels that leave no graph behind them.
+void require_once(const char* name) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), name, ": no second derivatives (backward was called with create_graph=True)");
+}
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+Tensor value(const OptTensor& t) { return t.value_or(Tensor()); }
+OptTensor maybe(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+// A 16-byte boundary: what the vector and TMA loads of contiguous tensors need, and every fresh allocation has.
+Tensor aligned(const Tensor& t) {
+    return t.numel() && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) ? t.clone(at::MemoryFormat::Contiguous) : t;
+}
+Tensor offsets(const OptTensor& cu, int64_t B, const char* name) {
+    if (!given(cu)) return Tensor();
+    TORCH_CHECK_VALUE(B == 1, name, ": cu_seqlens go with one packed row, got a batch of ", B);
+    TORCH_CHECK_VALUE(cu->dim() == 1 && cu->numel() >= 1, name, ": cu_seqlens [N+1]");
+    TORCH_CHECK_TYPE(at::isIntegralType(cu->scalar_type(), false), name, ": cu_seqlens are integers");
+    return as(*cu, at::kInt);
+}
+// Elements between the token rows of [B,T,...] with dense rows of `inner` elements, or -1: not one distance, a copy is needed.
+int64_t row_stride(const Tensor& t, int64_t inner) {
+    const int64_t B = t.size(0), T = t.size(1);
+    if (t.numel() == 0) return inner;
+    int64_t want = 1;
+    for (int64_t d = t.dim() - 1; d >= 2; --d) {
+        if (t.size(d) != 1 && t.stride(d) != want) return -1;
+        want *= t.size(d);
+    }
+    const int64_t rs = T > 1 ? t.stride(1) : B > 1 ? t.stride(0) : inner;
+    if (rs < inner || (T > 1 && B > 1 && t.stride(0) != T * rs)) return -1;
+    return rs;
+}
+Tensor rows(const Tensor& t, int64_t inner, int64_t& stride) {
+    stride = row_stride(t, inner);
+    if (stride >= 0) return t;
+    stride = inner;
+    return t.contiguous();
+}
+
+// ---- state space scan -------------------------------------------------------------------------------------------
+struct Ssm {
+    Tensor q, k, v, gt, gt_bias, g, D, h0, cu;  // undefined where absent
+    int64_t qs = 0, ks = 0, vs = 0;
+    bool softplus = false;
+};
+palimpsa_ssm ssm_params(const Ssm& x) {
+    palimpsa_ssm a{};
+    a.struct_size = sizeof(a);
+    a.io_dtype = io_code(x.v.scalar_type()), a.gt_dtype = io_code(x.gt.scalar_type());
+    a.flags = x.softplus ? PALIMPSA_SSM_SOFTPLUS : 0;
+    const int64_t B = x.v.size(0), T = x.v.size(1);
+    a.num_seqs = (int)(x.cu.defined() ? x.cu.numel() - 1 : B);
+    a.H = (int)x.v.size(2), a.Hq = (int)x.q.size(2), a.K = (int)x.q.size(3), a.V = (int)x.v.size(3);
+    a.seq_len = x.cu.defined() ? 0 : T, a.total_tokens = B * T;
+    a.q_stride = x.qs, a.k_stride = x.ks, a.v_stride = x.vs;
+    a.q = ptr(x.q), a.k = ptr(x.k), a.v = ptr(x.v), a.gt = ptr(x.gt);
+    a.gt_bias = ptr<float>(x.gt_bias), a.g = ptr<float>(x.g), a.D = ptr<float>(x.D), a.h0 = ptr<float>(x.h0);
+    a.cu_seqlens = ptr<int32_t>(x.cu);
+    return a;
+}
+struct SsmOut {
+    Tensor o, h, saved;
+};
+SsmOut ssm_fwd(const Ssm& x, bool final, bool training) {
+    const at::Device dev = x.v.device();
+    c10::cuda::CUDAGuard on_device(dev);
+    palimpsa_ssm a = ssm_params(x);
+    SsmOut r;
+    r.o = empty(x.v.sizes(), x.v.scalar_type(), dev);
+    if (final) r.h = empty({a.num_seqs, a.H, a.V, a.K}, at::kFloat, dev);
+    const size_t bytes = palimpsa_ssm_saved_bytes(&a, training);
+    r.saved = empty({std::max<int64_t>((int64_t)bytes, 256)}, at::kByte, dev);
+    a.o = ptr(r.o), a.h_out = ptr<float>(r.h), a.saved = ptr(r.saved), a.saved_bytes = (size_t)r.saved.numel();
+    check_rc(palimpsa_ssm_fwd(&a, training, stream_of(x.v)), "state space scan");
+    return r;
+}
+struct SsmFn : torch::autograd::Function<SsmFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gt,
+                                 const OptTensor& bias_, const Tensor& g, const OptTensor& D_, const OptTensor& h0_, const Ssm& rest,
+                                 bool final) {
+        const Tensor gt_bias = value(bias_), D = value(D_), h0 = value(h0_);
+        Ssm x{q, k, v, gt, gt_bias, g, D, h0, rest.cu, rest.qs, rest.ks, rest.vs, rest.softplus};
+        SsmOut r = ssm_fwd(x, final, true);
+        ctx->save_for_backward({q, k, v, gt, gt_bias, g, D, h0, rest.cu, r.saved});
+        ctx->saved_data["strides"] = std::vector<int64_t>{rest.qs, rest.ks, rest.vs, rest.softplus ? 1 : 0};
+        ctx->set_materialize_grads(false);
+        variable_list out{r.o};
+        if (final) out.push_back(r.h);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        require_once("chunk_ssm");
+        auto t = ctx->get_saved_variables();
+        const auto st = ctx->saved_data["strides"].toIntVector();
+        Ssm x{t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], st[0], st[1], st[2], st[3] != 0};
+        const at::Device dev = x.v.device();
+        const at::ScalarType io = x.v.scalar_type();
+        c10::cuda::CUDAGuard on_device(dev);
+        palimpsa_ssm a = ssm_params(x);
+        const Tensor d_o = aligned(grad_in(grads[0], x.v.sizes(), io, dev));
+        Tensor dh;
+        if (grads.size() > 1 && grads[1].defined()) dh = aligned(as(grads[1], at::kFloat));
+        Tensor dq = empty(x.q.sizes(), io, dev), dk = empty(x.k.sizes(), io, dev), dv = empty(x.v.sizes(), io, dev);
+        Tensor dgt = empty(x.gt.sizes(), x.gt.scalar_type(), dev), dg = empty({a.H}, at::kFloat, dev), db, dD, dh0;
+        if (x.gt_bias.defined()) db = empty({a.H}, at::kFloat, dev);
+        if (x.D.defined()) dD = empty({a.H}, at::kFloat, dev);
+        // the node's edges are those of the tensors that were given
+        const size_t h0_edge = 5 + (x.gt_bias.defined() ? 1 : 0) + (x.D.defined() ? 1 : 0);
+        if (x.h0.defined() && ctx->needs_input_grad(h0_edge)) dh0 = empty(x.h0.sizes(), at::kFloat, dev);
+        a.saved = ptr(t[9]), a.saved_bytes = (size_t)t[9].numel();
+        a.d_o = ptr(d_o), a.dh_out = ptr<float>(dh);
+        a.dq = ptr(dq), a.dk = ptr(dk), a.dv = ptr(dv), a.dgt = ptr(dgt);
+        a.dgt_bias = ptr<float>(db), a.dg = ptr<float>(dg), a.dD = ptr<float>(dD), a.dh0 = ptr<float>(dh0);
+        Tensor ws = empty({std::max<int64_t>((int64_t)palimpsa_ssm_workspace_bytes(&a), 256)}, at::kByte, dev);
+        a.workspace = ptr(ws), a.workspace_bytes = (size_t)ws.numel();
+        check_rc(palimpsa_ssm_bwd(&a, stream_of(x.v)), "state space scan backward");
+        return {dq, dk, dv, dgt, db, dg, dD, dh0, Tensor(), Tensor()};
+    }
+};
+
+// What chunk_ssm and ssm_step ask of their arguments, and the forms the kernels read.
+Ssm ssm_inputs(const char* name, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gt, const Tensor& g, const OptTensor& D,
+               const OptTensor& gt_bias, bool softplus, const OptTensor& state, const OptTensor& cu) {
+    const Tensor D_ = value(D), b_ = value(gt_bias), s_ = value(state), c_ = value(cu);
+    require_plain(name, {&q, &k, &v, &gt, &g, &D_, &b_, &s_, &c_});
+    require_same_device(name, v, {{"q", &q}, {"k", &k}, {"gt", &gt}, {"g", &g}, {"D", &D_}, {"gt_bias", &b_}, {"the state", &s_}, {"cu_seqlens", &c_}});
+    TORCH_CHECK_VALUE(q.dim() == 4 && q.sizes() == k.sizes() && v.dim() == 4 && q.size(0) == v.size(0) && q.size(1) == v.size(1),
+                      name, ": expected q,k [B,T,Hq,K] and v [B,T,H,V]");
+    const int64_t B = v.size(0), T = v.size(1), H = v.size(2), V = v.size(3), Hq = q.size(2), K = q.size(3);
+    TORCH_CHECK_VALUE(H > 0 && V > 0 && Hq > 0 && K > 0 && H % Hq == 0, name, ": H must be a multiple of Hq, and no head empty");
+    TORCH_CHECK_VALUE(K <= 256, name, ": d_k = ", K, " is above the supported maximum of 256");
+    TORCH_CHECK_VALUE(V <= 4096, name, ": d_v = ", V, " is above the supported maximum of 4096");
+    TORCH_CHECK_VALUE(gt.sizes() == at::IntArrayRef({B, T, H}) && g.numel() == H, name, ": expected gt [B,T,H] and g [H]");
+    TORCH_CHECK_VALUE((!given(D) || D->numel() == H) && (!given(gt_bias) || gt_bias->numel() == H), name, ": expected D and gt_bias [H]");
+    for (const Tensor* t : {&g, &D_, &b_, &s_})
+        TORCH_CHECK_TYPE(!t->defined() || t->is_floating_point(), name, ": g, D, gt_bias and the state are floating point");
+    at::ScalarType io = v.scalar_type();
+    for (const Tensor* t : {&q, &k}) io = c10::promoteTypes(io, t->scalar_type());
+    io_code(io), io_code(gt.scalar_type()), io_code(v.scalar_type());
+    Ssm x;
+    auto cast = [io](const Tensor& t) { return t.scalar_type() == io ? t : t.to(io); };
+    x.q = rows(cast(q), Hq * K, x.qs), x.k = rows(cast(k), Hq * K, x.ks), x.v = rows(cast(v), H * V, x.vs);
+    x.gt = dense(gt), x.g = as(g, at::kFloat).reshape({H});
+    if (given(D)) x.D = as(D_, at::kFloat).reshape({H});
+    if (given(gt_bias)) x.gt_bias = as(b_, at::kFloat).reshape({H});
+    x.softplus = softplus;
+    x.cu = offsets(cu, B, name);
+    return x;
+}
+
+py::object chunk_ssm(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& gt, const Tensor& g, const OptTensor& D,
+                     const OptTensor& gt_bias, bool softplus, const OptTensor& h0, bool final, const OptTensor& cu) {
+    Tensor o, h;
+    {
+        py::gil_scoped_release no_gil;
+        Ssm x = ssm_inputs("chunk_ssm", q, k, v, gt, g, D, gt_bias, softplus, h0, cu);
+        const int64_t N = x.cu.defined() ? x.cu.numel() - 1 : v.size(0);
+        if (given(h0)) {
+            TORCH_CHECK_VALUE(h0->sizes() == at::IntArrayRef({N, v.size(2), v.size(3), q.size(3)}), "chunk_ssm: initial_state must have shape (",
+                              N, ", ", v.size(2), ", ", v.size(3), ", ", q.size(3), ")");
+            x.h0 = as(*h0, at::kFloat);
+        }
+        RECORD_FUNCTION("palimpsa_b200::chunk_ssm", c10::ArrayRef<const c10::IValue>{});
+        if (wants_grad({&x.q, &x.k, &x.v, &x.gt, &x.gt_bias, &x.g, &x.D, &x.h0})) {
+            auto r = SsmFn::apply(x.q, x.k, x.v, x.gt, maybe(x.gt_bias), x.g, maybe(x.D), maybe(x.h0), x, final);
+            o = r[0];
+            if (final) h = r[1];
+        } else {
+            SsmOut r = ssm_fwd(x, final, false);
+            o = r.o, h = r.h;
+        }
+        if (o.scalar_type() != v.scalar_type()) o = o.to(v.scalar_type());
+    }
+    if (final) return py::make_tuple(o, h);
+    return py::cast(o);
+}
+
+Tensor ssm_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& gt_, const Tensor& g, const Tensor& state, const OptTensor& D,
+                const OptTensor& gt_bias, bool softplus) {
+    at::NoGradGuard no_grad;
+    const bool flat = v_.dim() == 3;
+    auto token = [flat](const Tensor& t) { return flat ? t.unsqueeze(1) : t; };
+    Ssm x = ssm_inputs("ssm_step", token(q_), token(k_), token(v_), token(gt_), g, D, gt_bias, softplus, state, std::nullopt);
+    const int64_t N = x.v.size(0), H = x.v.size(2), V = x.v.size(3), K = x.q.size(3);
+    TORCH_CHECK_VALUE(x.v.size(1) == 1, "ssm_step takes exactly one token per sequence");
+    TORCH_CHECK_VALUE(state.scalar_type() == at::kFloat && state.is_contiguous() && state.sizes() == at::IntArrayRef({N, H, V, K}),
+                      "ssm_step: the state must be contiguous float32 of shape (", N, ", ", H, ", ", V, ", ", K, ")");
+    TORCH_CHECK_VALUE(!(state.requires_grad() && state.is_leaf()), "ssm_step updates the state in place: it cannot be a leaf that requires grad");
+    c10::cuda::CUDAGuard on_device(x.v.device());
+    Tensor o = empty({N, 1, H, V}, x.v.scalar_type(), x.v.device());
+    palimpsa_ssm a = ssm_params(x);
+    a.h0 = ptr<float>(state), a.h_out = ptr<float>(state), a.o = ptr(o);
+    RECORD_FUNCTION("palimpsa_b200::ssm_step", c10::ArrayRef<const c10::IValue>{});
+    check_rc(palimpsa_ssm_step(&a, stream_of(x.v)), "state space step");
+    bump_version(state);
+    return o.scalar_type() == v_.scalar_type() ? o : o.to(v_.scalar_type());
+}
+
+// ---- short convolution --------------------------------------------------------------------------------------------
+struct Conv {
+    Tensor x, weight, bias, state, cu;
+    int64_t xs = 0;
+    bool silu = true;
+};
+palimpsa_short_conv conv_params(const Conv& c) {
+    palimpsa_short_conv a{};
+    a.struct_size = sizeof(a);
+    a.io_dtype = io_code(c.x.scalar_type());
+    a.W = (int)c.weight.size(1), a.flags = c.silu ? PALIMPSA_CONV_SILU : 0;
+    const int64_t B = c.x.size(0), T = c.x.size(1);
+    a.num_seqs = (int)(c.cu.defined() ? c.cu.numel() - 1 : B);
+    a.D = c.x.size(2), a.seq_len = c.cu.defined() ? 0 : T, a.total_tokens = B * T, a.x_stride = c.xs;
+    a.x = ptr(c.x), a.weight = ptr<float>(c.weight), a.bias = ptr<float>(c.bias), a.state = ptr(c.state), a.cu_seqlens = ptr<int32_t>(c.cu);
+    return a;
+}
+std::pair<Tensor, Tensor> conv_fwd(const Conv& c, bool final) {
+    c10::cuda::CUDAGuard on_device(c.x.device());
+    palimpsa_short_conv a = conv_params(c);
+    Tensor y = empty(c.x.sizes(), c.x.scalar_type(), c.x.device()), last;
+    if (final) last = empty({a.num_seqs, a.D, a.W - 1}, c.x.scalar_type(), c.x.device());
+    a.y = ptr(y), a.state_out = ptr(last);
+    check_rc(palimpsa_short_conv_fwd(&a, stream_of(c.x)), "short convolution");
+    return {y, last};
+}
+struct ConvFn : torch::autograd::Function<ConvFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias_, const OptTensor& state_,
+                                 const Conv& rest, bool final) {
+        const Tensor bias = value(bias_), state = value(state_);
+        auto [y, last] = conv_fwd({x, weight, bias, state, rest.cu, rest.xs, rest.silu}, final);
+        ctx->save_for_backward({x, weight, bias, state, rest.cu});
+        ctx->saved_data["misc"] = std::vector<int64_t>{rest.xs, rest.silu ? 1 : 0};
+        ctx->set_materialize_grads(false);
+        variable_list out{y};
+        if (final) out.push_back(last);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        require_once("short_conv");
+        auto t = ctx->get_saved_variables();
+        const auto misc = ctx->saved_data["misc"].toIntVector();
+        Conv c{t[0], t[1], t[2], t[3], t[4], misc[0], misc[1] != 0};
+        const at::Device dev = c.x.device();
+        const at::ScalarType io = c.x.scalar_type();
+        c10::cuda::CUDAGuard on_device(dev);
+        palimpsa_short_conv a = conv_params(c);
+        const Tensor dy = grad_in(grads[0], c.x.sizes(), io, dev);
+        Tensor dlast;
+        if (grads.size() > 1 && grads[1].defined()) dlast = as(grads[1], io);
+        Tensor dx = empty(c.x.sizes(), io, dev), dw = empty({a.D, a.W}, at::kFloat, dev), db, ds;
+        if (c.bias.defined()) db = empty({a.D}, at::kFloat, dev);
+        if (c.state.defined() && ctx->needs_input_grad(c.bias.defined() ? 3 : 2)) ds = empty(c.state.sizes(), io, dev);
+        a.dy = ptr(dy), a.dstate_out = ptr(dlast), a.dx = ptr(dx), a.dweight = ptr<float>(dw), a.dbias = ptr<float>(db), a.dstate = ptr(ds);
+        Tensor ws = empty({(int64_t)palimpsa_short_conv_workspace_bytes(&a)}, at::kByte, dev);
+        a.workspace = ptr(ws), a.workspace_bytes = (size_t)ws.numel();
+        check_rc(palimpsa_short_conv_bwd(&a, stream_of(c.x)), "short convolution backward");
+        return {dx, dw, db, ds, Tensor(), Tensor()};
+    }
+};
+Conv conv_inputs(const char* name, const Tensor& x, const Tensor& weight, const OptTensor& bias, bool silu, const OptTensor& state,
+                 const OptTensor& cu) {
+    const Tensor b_ = value(bias), s_ = value(state), c_ = value(cu);
+    require_plain(name, {&x, &weight, &b_, &s_, &c_});
+    require_same_device(name, x, {{"weight", &weight}, {"bias", &b_}, {"the state", &s_}, {"cu_seqlens", &c_}});
+    io_code(x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() == 3 && x.size(2) > 0, name, ": expected x [B,T,D]");
+    const int64_t D = x.size(2);
+    TORCH_CHECK_VALUE((weight.dim() == 2 || (weight.dim() == 3 && weight.size(1) == 1)) && weight.size(0) == D, name,
+                      ": expected weight [D,W] or [D,1,W]");
+    const int64_t W = weight.size(-1);
+    TORCH_CHECK_VALUE(W >= 2 && W <= 4, name, ": a width of ", W, " is not supported (2 to 4)");
+    TORCH_CHECK_VALUE(!given(bias) || bias->numel() == D, name, ": expected bias [D]");
+    TORCH_CHECK_TYPE(weight.is_floating_point() && (!given(bias) || bias->is_floating_point()), name, ": weight and bias are floating point");
+    Conv c;
+    c.x = rows(x, D, c.xs);
+    c.weight = as(weight, at::kFloat).reshape({D, W});
+    if (given(bias)) c.bias = as(b_, at::kFloat).reshape({D});
+    c.cu = offsets(cu, x.size(0), name);
+    c.silu = silu;
+    return c;
+}
+py::object short_conv(const Tensor& x, const Tensor& weight, const OptTensor& bias, bool silu, const OptTensor& state, bool final,
+                      const OptTensor& cu) {
+    Tensor y, last;
+    {
+        py::gil_scoped_release no_gil;
+        Conv c = conv_inputs("short_conv", x, weight, bias, silu, state, cu);
+        if (given(state)) {
+            const int64_t N = c.cu.defined() ? c.cu.numel() - 1 : x.size(0), D = x.size(2), W1 = c.weight.size(1) - 1;
+            TORCH_CHECK_VALUE(state->sizes() == at::IntArrayRef({N, D, W1}), "short_conv: initial_state must have shape (", N, ", ", D, ", ", W1, ")");
+            c.state = as(*state, x.scalar_type());
+        }
+        RECORD_FUNCTION("palimpsa_b200::short_conv", c10::ArrayRef<const c10::IValue>{});
+        if (wants_grad({&c.x, &c.weight, &c.bias, &c.state})) {
+            auto r = ConvFn::apply(c.x, c.weight, maybe(c.bias), maybe(c.state), c, final);
+            y = r[0];
+            if (final) last = r[1];
+        } else {
+            std::tie(y, last) = conv_fwd(c, final);
+        }
+    }
+    if (final) return py::make_tuple(y, last);
+    return py::cast(y);
+}
+Tensor short_conv_step(const Tensor& x_, const Tensor& weight, const Tensor& state, const OptTensor& bias, bool silu) {
+    at::NoGradGuard no_grad;
+    const bool flat = x_.dim() == 2;
+    Conv c = conv_inputs("short_conv_step", flat ? x_.unsqueeze(1) : x_, weight, bias, silu, state, std::nullopt);
+    const int64_t N = c.x.size(0), D = c.x.size(2), W1 = c.weight.size(1) - 1;
+    TORCH_CHECK_VALUE(c.x.size(1) == 1, "short_conv_step takes exactly one token per sequence");
+    TORCH_CHECK_VALUE(state.scalar_type() == c.x.scalar_type() && state.is_contiguous() && state.sizes() == at::IntArrayRef({N, D, W1}),
+                      "short_conv_step: the state must be contiguous ", c.x.scalar_type(), " of shape (", N, ", ", D, ", ", W1, ")");
+    TORCH_CHECK_VALUE(!(state.requires_grad() && state.is_leaf()), "short_conv_step updates the state in place: it cannot be a leaf that requires grad");
+    c10::cuda::CUDAGuard on_device(c.x.device());
+    Tensor y = empty(x_.sizes(), c.x.scalar_type(), c.x.device());
+    palimpsa_short_conv a = conv_params(c);
+    a.state = ptr(state), a.state_out = ptr(state), a.y = ptr(y);
+    RECORD_FUNCTION("palimpsa_b200::short_conv_step", c10::ArrayRef<const c10::IValue>{});
+    check_rc(palimpsa_short_conv_step(&a, stream_of(c.x)), "short convolution step");
+    bump_version(state);
+    return y;
+}
+
+// ---- residual norm --------------------------------------------------------------------------------------------------
+struct Norm {
+    Tensor x, res, weight;
+    int64_t xs = 0;
+    double eps = 1e-5;
+};
+// Elements between the rows of [...,D], or -1.
+int64_t last_row_stride(const Tensor& t) {
+    const int64_t D = t.size(-1);
+    if (t.is_contiguous()) return D;
+    if (t.stride(-1) != 1 && D != 1) return -1;
+    int64_t rs = -1, want = -1;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (rs < 0) rs = t.stride(d);
+        else if (t.stride(d) != want) return -1;
+        want = t.stride(d) * t.size(d);
+    }
+    return rs >= D ? rs : -1;
+}
+palimpsa_rms_norm norm_params(const Norm& n) {
+    palimpsa_rms_norm a{};
+    a.struct_size = sizeof(a);
+    a.io_dtype = io_code(n.x.scalar_type());
+    a.res_dtype = n.res.defined() ? io_code(n.res.scalar_type()) : -1;
+    a.D = n.x.size(-1), a.rows = n.x.numel() / a.D, a.x_stride = n.xs, a.eps = n.eps;
+    a.x = ptr(n.x), a.res = ptr(n.res), a.weight = ptr<float>(n.weight);
+    return a;
+}
+std::pair<Tensor, Tensor> norm_fwd(const Norm& n) {
+    const at::Device dev = n.x.device();
+    c10::cuda::CUDAGuard on_device(dev);
+    palimpsa_rms_norm a = norm_params(n);
+    Tensor y = empty(n.x.sizes(), n.x.scalar_type(), dev), z;
+    if (n.res.defined()) z = empty(n.x.sizes(), n.res.scalar_type(), dev);
+    a.y = ptr(y), a.z = ptr(z);
+    check_rc(palimpsa_rms_norm_fwd(&a, stream_of(n.x)), "residual norm");
+    return {y, z};
+}
+struct NormFn : torch::autograd::Function<NormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& res_, const Tensor& weight, int64_t xs, double eps) {
+        const Tensor res = value(res_);
+        auto [y, z] = norm_fwd({x, res, weight, xs, eps});
+        ctx->save_for_backward({res.defined() ? z : x, weight});
+        ctx->saved_data["types"] = pack_dtypes({x.scalar_type(), res.defined() ? res.scalar_type() : x.scalar_type()});
+        ctx->saved_data["misc"] = std::vector<int64_t>{xs, res.defined() ? 1 : 0};
+        ctx->saved_data["eps"] = eps;
+        ctx->set_materialize_grads(false);
+        if (res.defined()) return {y, z};
+        return {y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        require_once("add_rms_norm");
+        auto t = ctx->get_saved_variables();
+        const int64_t types = ctx->saved_data["types"].toInt();
+        const auto misc = ctx->saved_data["misc"].toIntVector();
+        const at::ScalarType io = dtype_at(types, 0), rt = dtype_at(types, 1);
+        const bool has_res = misc[1] != 0;
+        const Tensor& z = t[0];
+        const at::Device dev = z.device();
+        c10::cuda::CUDAGuard on_device(dev);
+        palimpsa_rms_norm a{};
+        a.struct_size = sizeof(a);
+        a.io_dtype = io_code(io), a.res_dtype = has_res ? io_code(rt) : -1;
+        a.D = z.size(-1), a.rows = z.numel() / a.D, a.x_stride = misc[0], a.eps = ctx->saved_data["eps"].toDouble();
+        a.weight = ptr<float>(t[1]);
+        if (has_res) a.z = ptr(z);
+        else a.x = ptr(z);
+        const Tensor dy = grad_in(grads[0], z.sizes(), io, dev);
+        Tensor dz, dx = empty(z.sizes(), io, dev), dres, dw = empty({a.D}, at::kFloat, dev);
+        if (has_res && grads[1].defined()) dz = as(grads[1], rt);
+        if (has_res && rt != io) dres = empty(z.sizes(), rt, dev);
+        a.dy = ptr(dy), a.dz = ptr(dz), a.dx = ptr(dx), a.dres = ptr(dres), a.dweight = ptr<float>(dw);
+        Tensor ws = empty({(int64_t)palimpsa_rms_norm_workspace_bytes(&a)}, at::kByte, dev);
+        a.workspace = ptr(ws), a.workspace_bytes = (size_t)ws.numel();
+        check_rc(palimpsa_rms_norm_bwd(&a, stream_of(z)), "residual norm backward");
+        if (has_res && rt == io) dres = dx;  // as an addition hands its gradient to both sides
+        return {dx, dres, dw, Tensor(), Tensor()};
+    }
+};
+Norm norm_inputs(const char* name, const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps) {
+    const Tensor r_ = value(residual);
+    require_plain(name, {&x, &weight, &r_});
+    require_same_device(name, x, {{"weight", &weight}, {"residual", &r_}});
+    io_code(x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && weight.numel() == x.size(-1), name, ": expected x [...,D] and weight [D]");
+    TORCH_CHECK_VALUE(x.size(-1) <= 16384, name, ": D = ", x.size(-1), " is above the supported maximum of 16384");
+    TORCH_CHECK_VALUE(!given(residual) || residual->sizes() == x.sizes(), name, ": expected a residual like x");
+    TORCH_CHECK_VALUE(eps >= 0, name, ": eps must not be negative");
+    TORCH_CHECK_TYPE(weight.is_floating_point(), name, ": the weight is floating point");
+    if (given(residual))
+        TORCH_CHECK_TYPE(residual->scalar_type() == x.scalar_type() || residual->scalar_type() == at::kFloat, name,
+                         ": the residual must have x's type or float32, got ", residual->scalar_type(), " beside ", x.scalar_type());
+    Norm n;
+    n.xs = last_row_stride(x);
+    n.x = n.xs >= 0 ? x : x.contiguous();
+    if (n.xs < 0) n.xs = x.size(-1);
+    if (given(residual)) n.res = dense(r_);
+    n.weight = as(weight, at::kFloat).reshape({x.size(-1)});
+    n.eps = eps;
+    return n;
+}
+std::pair<Tensor, Tensor> add_rms_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps) {
+    Norm n = norm_inputs("add_rms_norm", x, weight, residual, eps);
+    RECORD_FUNCTION("palimpsa_b200::add_rms_norm", c10::ArrayRef<const c10::IValue>{});
+    if (wants_grad({&n.x, &n.res, &n.weight})) {
+        auto r = NormFn::apply(n.x, maybe(n.res), n.weight, n.xs, n.eps);
+        return {r[0], n.res.defined() ? r[1] : x};
+    }
+    auto [y, z] = norm_fwd(n);
+    return {y, n.res.defined() ? z : x};
+}
+std::tuple<Tensor, Tensor, Tensor> add_rms_norm_quant(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps,
+                                                      at::ScalarType type, int64_t block) {
+    TORCH_CHECK_TYPE(type == at::kFloat8_e4m3fn || type == at::kChar, "add_rms_norm_quant: dtype must be float8_e4m3fn or int8, got ", type);
+    TORCH_CHECK_VALUE(block == 0 || block == 32 || block == 64 || block == 128 || block == 256,
+                      "add_rms_norm_quant: block must be None, 32, 64, 128 or 256, got ", block);
+    Norm n = norm_inputs("add_rms_norm_quant", x, weight, residual, eps);
+    TORCH_CHECK(!wants_grad({&n.x, &n.res, &n.weight}), "add_rms_norm_quant has no gradient: call it under torch.no_grad()");
+    const at::Device dev = x.device();
+    c10::cuda::CUDAGuard on_device(dev);
+    palimpsa_rms_norm a = norm_params(n);
+    a.out_type = type == at::kChar ? PALIMPSA_NORM_INT8 : PALIMPSA_NORM_E4M3;
+    a.block = (int)block;
+    auto scales = x.sizes().vec();
+    scales.back() = block ? (a.D + block - 1) / block : 1;
+    Tensor y = empty(x.sizes(), type, dev), s = empty(scales, at::kFloat, dev), z;
+    if (n.res.defined()) z = empty(x.sizes(), n.res.scalar_type(), dev);
+    a.y = ptr(y), a.z = ptr(z), a.scale = ptr<float>(s);
+    RECORD_FUNCTION("palimpsa_b200::add_rms_norm_quant", c10::ArrayRef<const c10::IValue>{});
+    check_rc(palimpsa_rms_norm_fwd(&a, stream_of(x)), "residual norm");
+    return {y, s, n.res.defined() ? z : x};
+}
+
+}  // namespace
+
+void def_block_operators(py::module_& m) {
+    using no_gil = py::call_guard<py::gil_scoped_release>;
+    m.def("chunk_ssm", &chunk_ssm);
+    m.def("ssm_step", &ssm_step, no_gil());
+    m.def("short_conv", &short_conv);
+    m.def("short_conv_step", &short_conv_step, no_gil());
+    m.def("add_rms_norm", &add_rms_norm, no_gil());
+    m.def("add_rms_norm_quant",
+          [](const Tensor& x, const Tensor& w, const OptTensor& r, double eps, py::object dtype, int64_t block) {
+              const at::ScalarType t = torch::python::detail::py_object_to_dtype(dtype);
+              py::gil_scoped_release release;
+              return add_rms_norm_quant(x, w, r, eps, t, block);
+          });
+}
+
+}  // namespace palimpsa_torch

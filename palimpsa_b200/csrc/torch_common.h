@@ -1,0 +1,112 @@
+// What the files of the torch front end share: argument checks, dtype policy, allocation.
+#pragma once
+
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <ATen/record_function.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/extension.h>
+#include <torch/library.h>
+
+#include <array>
+#include <optional>
+#include <tuple>
+
+#include "../../include/palimpsa_b200.h"
+
+namespace palimpsa_torch {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+inline void check_rc(int rc, const char* what) {
+    TORCH_CHECK(rc == PALIMPSA_OK, what, " failed with code ", rc, ": ", palimpsa_last_error_string(rc));
+}
+inline bool supported_dtype(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+inline int io_code(at::ScalarType t) {
+    TORCH_CHECK_TYPE(supported_dtype(t), "unsupported dtype ", t, "; use float32, bfloat16 or float16");
+    return t == at::kFloat ? PALIMPSA_F32 : (t == at::kBFloat16 ? PALIMPSA_BF16 : PALIMPSA_F16);
+}
+inline Tensor empty(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
+    return at::detail::empty_cuda(sizes, dt, dev, std::nullopt);
+}
+inline Tensor none_like(const Tensor& t, at::ScalarType dt) { return at::empty({0}, t.options().dtype(dt)); }
+template <class T = void>
+T* ptr(const Tensor& t) {
+    return t.defined() && t.numel() ? static_cast<T*>(const_cast<void*>(t.const_data_ptr())) : nullptr;
+}
+template <class T = void>
+T* ptr(const OptTensor& t) {
+    return t ? ptr<T>(*t) : nullptr;
+}
+inline bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+inline void require_cuda(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK(!t->defined() || t->is_cuda(),
+                    "palimpsa_b200 runs on CUDA (sm_100a) only and has no CPU path; for CPU tensors use "
+                    "palimpsa_b200.ops.palimpsa_ref (naive recurrence).");
+}
+// The last check before pointers are taken, whichever way a call came in: the kernels read each argument through a raw
+// pointer, so a host tensor, one of another GPU, another dtype, length or stride would be a fault or garbage there.
+inline void check_arg(const char* name, const Tensor& t, at::ScalarType dt, at::IntArrayRef sizes, const at::Device& dev) {
+    if (!t.defined()) return;
+    require_cuda({&t});
+    TORCH_CHECK_VALUE(t.device() == dev, name, " is on ", t.device(), ", q on ", dev);
+    TORCH_CHECK_TYPE(t.scalar_type() == dt, name, " has dtype ", t.scalar_type(), ", expected ", dt);
+    TORCH_CHECK_VALUE(t.numel() == c10::multiply_integers(sizes), name, " has shape ", t.sizes(), ", expected ", sizes);
+    TORCH_CHECK_VALUE(t.is_contiguous(), name, " is not contiguous");
+}
+// Nothing between the caller and the kernels: dense CUDA tensors and the thread's usual dispatch state.  Everything else
+// (a mode, a transform, a tracer, a fake, negated, batched or wrapped tensor, a kernel that runs below autograd) has a
+// dispatch key of its own, on the thread or on the tensor, and goes through the registered operators, which is where those
+// hook in.  Named by what is allowed, so that a key nobody thought of takes the general route.
+inline bool plain(std::initializer_list<const Tensor*> ts) {
+    using c10::DispatchKey;
+    using c10::DispatchKeySet;
+    // bits, not key-set differences: those leave a set's backends standing
+    static const uint64_t usual_state = (c10::default_included_set | c10::autocast_dispatch_keyset).raw_repr();
+    static const uint64_t usual_tensor = (DispatchKeySet(DispatchKey::CUDA) | DispatchKeySet(DispatchKey::AutogradCUDA) |
+                                          DispatchKeySet(DispatchKey::ADInplaceOrView) | DispatchKeySet(DispatchKey::AutocastCUDA))
+                                             .raw_repr();
+    if (c10::impl::dispatch_mode_enabled()) return false;
+    const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
+    if (tls.included_.raw_repr() & ~usual_state) return false;
+    // below autograd no node may be made (inference mode is there too, with gradients off: nothing to make)
+    if (at::GradMode::is_enabled() && (tls.excluded_.raw_repr() & c10::autograd_dispatch_keyset.raw_repr())) return false;
+    for (const Tensor* t : ts)
+        if (t->defined() && (t->key_set().raw_repr() & ~usual_tensor)) return false;
+    return true;
+}
+inline py::object not_plain() { return py::reinterpret_borrow<py::object>(Py_NotImplemented); }  // the caller takes the general route
+inline Tensor as(const Tensor& t, at::ScalarType dt) {
+    Tensor r = t.scalar_type() == dt ? t : t.to(dt);
+    return r.is_contiguous() ? r : r.contiguous();
+}
+inline Tensor as_opt(const OptTensor& t, at::ScalarType dt) { return given(t) ? as(*t, dt) : Tensor(); }
+inline Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+inline Tensor dense(const OptTensor& t) { return given(t) ? dense(*t) : Tensor(); }
+inline void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+inline void bump_version(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// The dtypes of the arguments as the caller passed them, a byte each (a value that hashes: see the operator's node).
+inline int64_t pack_dtypes(std::initializer_list<at::ScalarType> ts) {
+    int64_t bits = 0, shift = 0;
+    for (at::ScalarType t : ts) bits |= static_cast<int64_t>(t) << shift, shift += 8;
+    return bits;
+}
+inline at::ScalarType dtype_at(int64_t bits, size_t i) { return static_cast<at::ScalarType>(bits >> (8 * i) & 0xff); }
+inline Tensor grad_in(const Tensor& g, at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
+    return g.defined() ? as(g, dt) : at::zeros(sizes, at::TensorOptions().dtype(dt).device(dev));
+}
+
+// The operators of the block around the recurrence (torch_block.cpp).
+void def_block_operators(pybind11::module_& m);
+
+}  // namespace palimpsa_torch

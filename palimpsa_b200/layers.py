@@ -9,11 +9,16 @@ element-wise passes (palimpsa/layers/palimpsa.py:266-281 and :337-343).  :func:`
     o = layer_epilogue(o, x, self.D, self.o_norm.weight, gate, eps=self.o_norm.eps)
 
 Both are differentiable (autograd nodes of the native front end over the C ABI) and run on CUDA only.
+
+What the layers and blocks have around that, and take from flash-linear-attention in the reference, is here too:
+:func:`short_conv` (with :func:`short_conv_step` for decoding) in front of q, k and v, and :func:`add_rms_norm` (with
+:func:`add_rms_norm_quant` for 8-bit projections) between the blocks.
 """
 from __future__ import annotations
 
 from typing import Optional
 
+import torch
 from torch import Tensor
 
 from .ops.palimpsa import _core
@@ -39,3 +44,49 @@ def layer_epilogue(o: Tensor, x: Optional[Tensor], D: Optional[Tensor], weight: 
     norm of flash-linear-attention's ``FusedRMSNormGated``, activation "swish").  float32 arithmetic, result
     in ``o.dtype``."""
     return (_core._native or _core.native()).layer_epilogue(o, x, D, weight, gate, float(eps))
+
+
+def _silu(activation) -> bool:
+    if activation not in (None, "silu", "swish"):
+        raise ValueError(f"activation must be None, 'silu' or 'swish', got {activation!r}")
+    return activation is not None
+
+
+def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = "silu",
+               initial_state: Optional[Tensor] = None, output_final_state: bool = False,
+               cu_seqlens: Optional[Tensor] = None):
+    """Causal depthwise convolution over the last ``W`` tokens of each channel, then SiLU
+    (``activation=None``: without): ``y_t = act(bias + sum_w weight[:, w] * x_{t-(W-1)+w})``.
+
+    ``x [B, T, D]`` (token rows may lie apart, as in a slice of a wider projection), ``weight [D, W]`` or
+    ``[D, 1, W]`` with W = 2, 3 or 4, ``bias [D]``.  ``initial_state [N, D, W-1]`` holds the inputs in front of
+    each sequence, oldest first (zero without it); ``output_final_state`` also returns the last ones, in ``x.dtype``,
+    for :func:`short_conv_step`.  ``cu_seqlens [N+1]``: packed sequences in one row (B = 1); rows outside them are zero.
+    Differentiable in x, weight, bias and initial_state (once); float32 arithmetic, result in ``x.dtype``."""
+    return (_core._native or _core.native()).short_conv(x, weight, bias, _silu(activation), initial_state,
+                                                        bool(output_final_state), cu_seqlens)
+
+
+def short_conv_step(x: Tensor, weight: Tensor, state: Tensor, bias: Optional[Tensor] = None,
+                    activation: Optional[str] = "silu") -> Tensor:
+    """:func:`short_conv` for one token of each of N sequences: ``x [N, D]`` or ``[N, 1, D]``, ``state [N, D, W-1]``
+    (contiguous, x's dtype) UPDATED IN PLACE.  Returns y like x.  Not differentiable; can be captured in a CUDA graph."""
+    return (_core._native or _core.native()).short_conv_step(x, weight, state, bias, _silu(activation))
+
+
+def add_rms_norm(x: Tensor, weight: Tensor, residual: Optional[Tensor] = None, eps: float = 1e-5):
+    """The residual's addition and the RMS norm of a block: ``z = x + residual`` in the residual's dtype (x's or
+    float32), ``y = z * weight / sqrt(mean(z^2) + eps)`` over the last axis (at most 16384 channels), in ``x.dtype``.
+    Returns ``(y, z)``; without a residual z is x itself.  The norm is that of z as it is stored, i.e. of what the next
+    block adds to.  Differentiable in x, weight and residual (once)."""
+    return (_core._native or _core.native()).add_rms_norm(x, weight, residual, float(eps))
+
+
+def add_rms_norm_quant(x: Tensor, weight: Tensor, residual: Optional[Tensor] = None, eps: float = 1e-5,
+                       dtype: torch.dtype = torch.float8_e4m3fn, block: Optional[int] = None):
+    """:func:`add_rms_norm` with y in 8 bits (``torch.float8_e4m3fn`` or ``torch.int8``) for a product with 8-bit
+    weights.  Returns ``(q, scale, z)`` with y = q * scale: one float32 scale per row (``scale [..., 1]``), or per row
+    and ``block`` channels (32, 64, 128 or 256; ``scale [..., ceil(D / block)]``).  ``scale = max(amax |y|, 2^-100) / top``
+    with top = 448 or 127; q is the nearest 8-bit value of y / scale, ties to even, decided as in 64-bit arithmetic, so it
+    does not depend on how sums are ordered.  A row with a NaN gets NaN scales.  Not differentiable."""
+    return (_core._native or _core.native()).add_rms_norm_quant(x, weight, residual, float(eps), dtype, int(block or 0))

@@ -1,0 +1,44 @@
+"""The selective state space scan: the recurrence of the palimpsa operator without its precision state.
+
+The MetaMamba2 layer hands ``chunk_palimpsa`` C as q, B as k, x as v and dt as gt (palimpsa/layers/meta_mamba2.py:294-299);
+``chunk_ssm`` takes the same tensors for the plain scan, with q and k heads shared between value heads, the step size's
+bias and softplus and the skip term inside.  There is no fallback: CUDA tensors only.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+from torch import Tensor
+
+from .palimpsa import _core
+
+
+def chunk_ssm(q: Tensor, k: Tensor, v: Tensor, gt: Tensor, g: Tensor, D: Optional[Tensor] = None,
+              gt_bias: Optional[Tensor] = None, gt_softplus: bool = False, initial_state: Optional[Tensor] = None,
+              output_final_state: bool = False, cu_seqlens: Optional[Tensor] = None):
+    """Selective state space scan over whole sequences (training and prompts).  Per sequence and head, with
+    ``dt_t = gt_t``, or ``softplus(gt_t + gt_bias)`` with ``gt_softplus`` (the bias is added in either case)::
+
+        h_t = exp(-g * dt_t) * h_{t-1} + dt_t * v_t k_t^T          o_t = h_t q_t + D * v_t
+
+    ``q, k [B, T, Hq, K]`` (K <= 256), ``v [B, T, H, V]`` with H a multiple of Hq: head h reads q and k of head
+    ``h // (H // Hq)``.  ``gt [B, T, H]``, ``g, D, gt_bias [H]``; decays are meant to be at most 1 (g * dt >= 0).  Token
+    rows of q, k and v may lie apart (slices of one projection are read in place).  ``initial_state [N, H, V, K]``, zero
+    without it.  ``cu_seqlens [N+1]``: packed sequences in one row (B = 1); rows outside them get zeros.
+
+    Returns ``o [B, T, H, V]`` in v's dtype, and with ``output_final_state`` the float32 state after each sequence,
+    which :func:`ssm_step` goes on from.  Differentiable (once) in q, k, v, gt, g, D, gt_bias and initial_state,
+    also through the final state.  Results repeat bit by bit.
+
+    bfloat16 with K and V multiples of 8, K <= 128 and rows on 16-byte boundaries runs on the tensor cores: products of
+    bfloat16 operands summed in float32, the state in float32.  Everything else is float32 throughout."""
+    return (_core._native or _core.native()).chunk_ssm(q, k, v, gt, g, D, gt_bias, bool(gt_softplus), initial_state,
+                                                       bool(output_final_state), cu_seqlens)
+
+
+def ssm_step(q: Tensor, k: Tensor, v: Tensor, gt: Tensor, g: Tensor, state: Tensor, D: Optional[Tensor] = None,
+             gt_bias: Optional[Tensor] = None, gt_softplus: bool = False) -> Tensor:
+    """:func:`chunk_ssm` for one token of each of N sequences: ``q, k [N, 1, Hq, K]``, ``v [N, 1, H, V]``,
+    ``gt [N, 1, H]`` (or all without the 1), ``state [N, H, V, K]`` float32, contiguous, UPDATED IN PLACE.
+    Returns ``o [N, 1, H, V]``.  Not differentiable; can be captured in a CUDA graph."""
+    return (_core._native or _core.native()).ssm_step(q, k, v, gt, g, state, D, gt_bias, bool(gt_softplus))

@@ -1,0 +1,143 @@
+"""CPU checks of the operators around the recurrence: C structs, argument codes, refusals, and the oracle against differences."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+from oracle import block_oracle as bo
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "palimpsa_b200.h")
+
+
+@pytest.fixture(scope="module")
+def L():
+    from palimpsa_b200 import _lib
+    _lib.lib()
+    return _lib
+
+
+def test_struct_layout_matches_c(L, tmp_path):
+    pairs = (("palimpsa_ssm", L.Ssm), ("palimpsa_short_conv", L.ShortConv), ("palimpsa_rms_norm", L.RmsNorm))
+    lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{HEADER}"', "int main(){"]
+    for name, cls in pairs:
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        lines += [f'printf("%zu\\n", offsetof({name}, {f[0]}));' for f in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.check_call(["gcc", "-std=c99", "-Wall", "-Werror", str(src), "-o", str(tmp_path / "layout")])
+    it = iter(int(x) for x in subprocess.check_output([str(tmp_path / "layout")]).split())
+    for name, cls in pairs:
+        assert next(it) == C.sizeof(cls), name
+        for f in cls._fields_:
+            assert next(it) == getattr(cls, f[0]).offset, (name, f[0])
+
+
+def _ssm(L, **kw):
+    a = L.Ssm()
+    a.struct_size = C.sizeof(L.Ssm)
+    a.num_seqs, a.H, a.Hq, a.K, a.V, a.seq_len, a.total_tokens = 2, 4, 2, 16, 8, 5, 10
+    a.q_stride = a.k_stride = 32
+    a.v_stride = 32
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
+def test_ssm_argument_codes(L):
+    lib = L.lib()
+    call = lambda a: lib.palimpsa_ssm_fwd(C.byref(a), 0, None)
+    assert lib.palimpsa_ssm_fwd(None, 0, None) == -1 and lib.palimpsa_ssm_bwd(None, None) == -1
+    assert call(_ssm(L, struct_size=4)) == -8
+    assert call(_ssm(L, Hq=3)) == -2 and call(_ssm(L, total_tokens=11)) == -2 and call(_ssm(L, q_stride=31)) == -2
+    assert call(_ssm(L, K=257, q_stride=600, k_stride=600)) == -3 and call(_ssm(L, V=4097, v_stride=1 << 20)) == -3
+    assert call(_ssm(L, io_dtype=5)) == -4 and call(_ssm(L, gt_dtype=-1)) == -4
+    assert call(_ssm(L)) == -1                                        # no tensors
+    p = dict(q=4096, k=4096, v=4096, gt=4096, g=4096, o=4096)
+    assert call(_ssm(L, **p)) == -5                                   # no buffer for what is saved
+    assert call(_ssm(L, **p, saved=4096, saved_bytes=16)) == -5
+    assert call(_ssm(L, **p, saved=4097, saved_bytes=1 << 30)) == -5
+    assert lib.palimpsa_ssm_step(C.byref(_ssm(L, **p)), None) == -2   # more than a token per sequence
+    assert lib.palimpsa_ssm_step(C.byref(_ssm(L, **p, total_tokens=2, seq_len=1)), None) == -1
+    assert lib.palimpsa_ssm_saved_bytes(C.byref(_ssm(L)), 1) > 0 and lib.palimpsa_ssm_saved_bytes(None, 1) == 0
+    assert lib.palimpsa_ssm_workspace_bytes(C.byref(_ssm(L))) > 0
+    # an empty call launches nothing
+    assert call(_ssm(L, num_seqs=0, total_tokens=0, g=4096, saved=4096, saved_bytes=1 << 20)) == 0
+
+
+def test_conv_and_norm_argument_codes(L):
+    lib = L.lib()
+    a = L.ShortConv()
+    assert lib.palimpsa_short_conv_fwd(C.byref(a), None) == -8
+    a.struct_size = C.sizeof(L.ShortConv)
+    assert lib.palimpsa_short_conv_fwd(C.byref(a), None) == -2
+    a.D = a.x_stride = 8
+    a.num_seqs, a.seq_len, a.total_tokens, a.W = 1, 4, 4, 5
+    assert lib.palimpsa_short_conv_fwd(C.byref(a), None) == -3
+    a.W = 4
+    assert lib.palimpsa_short_conv_fwd(C.byref(a), None) == -1
+    a.x = a.weight = a.dy = a.dx = a.dweight = 4096
+    assert lib.palimpsa_short_conv_bwd(C.byref(a), None) == -5
+    n = L.RmsNorm()
+    n.struct_size = C.sizeof(L.RmsNorm)
+    n.rows, n.D, n.x_stride, n.res_dtype = 2, 16385, 16385, -1
+    assert lib.palimpsa_rms_norm_fwd(C.byref(n), None) == -3
+    n.D = n.x_stride = 16
+    n.block = 48
+    assert lib.palimpsa_rms_norm_fwd(C.byref(n), None) == -2
+    n.block, n.res_dtype = 0, 2
+    assert lib.palimpsa_rms_norm_fwd(C.byref(n), None) == -4          # a float16 residual beside float32
+    n.res_dtype = -1
+    assert lib.palimpsa_rms_norm_fwd(C.byref(n), None) == -1
+
+
+def test_python_entry_points_refuse_host_tensors_and_bad_arguments():
+    from palimpsa_b200.layers import add_rms_norm, add_rms_norm_quant, short_conv, short_conv_step
+    from palimpsa_b200.ops import chunk_ssm, ssm_step
+    q, v, gt, g = torch.randn(1, 4, 1, 8), torch.randn(1, 4, 2, 8), torch.rand(1, 4, 2), torch.ones(2)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        chunk_ssm(q, q, v, gt, g)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ssm_step(q[:, :1], q[:, :1], v[:, :1], gt[:, :1], g, torch.zeros(1, 2, 8, 8))
+    x, w = torch.randn(1, 4, 8), torch.randn(8, 4)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        short_conv(x, w)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        short_conv_step(x[:, 0], w, torch.zeros(1, 8, 3))
+    with pytest.raises(ValueError, match="activation"):
+        short_conv(x, w, activation="relu")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        add_rms_norm(x, torch.ones(8))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        add_rms_norm_quant(x, torch.ones(8))
+    with pytest.raises(TypeError, match="float8_e4m3fn or int8"):
+        add_rms_norm_quant(x, torch.ones(8), dtype=torch.float16)
+    with pytest.raises(ValueError, match="block"):
+        add_rms_norm_quant(x, torch.ones(8), block=100)
+
+
+def test_oracle_scan_gradients_match_differences():
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, dtype=torch.float64)
+    leaves = dict(q=r(1, 7, 1, 3), k=r(1, 7, 1, 3), v=r(1, 7, 2, 4), gt=r(1, 7, 2), g=r(2).abs(), D=r(2), gt_bias=r(2), h0=r(2, 2, 4, 3))
+    do, dh, cu = r(1, 7, 2, 4), r(2, 2, 4, 3), [1, 3, 7]
+    run = lambda **kw: bo.ssm(**{**leaves, **kw}, softplus=True, do=do, dh=dh, cu=cu)
+    loss = lambda out: float((out["o"] * do).sum() + (out["h"] * dh).sum())
+    grads = run()
+    for name, x in leaves.items():
+        for i in range(0, x.numel(), max(1, x.numel() // 5)):
+            step = torch.zeros_like(x).view(-1)
+            step[i] = 1e-5
+            step = step.view_as(x)
+            diff = (loss(run(**{name: x + step})) - loss(run(**{name: x - step}))) / 2e-5
+            assert abs(diff - float(grads["d" + name].reshape(-1)[i])) < 1e-7 * (1 + abs(diff)), (name, i)
+
+
+def test_oracle_rounds_to_eight_bits_as_torch_does():
+    y = torch.cat([torch.linspace(-448, 448, 4001, dtype=torch.float64), torch.linspace(-0.02, 0.02, 1001, dtype=torch.float64)])[None]
+    q, s = bo.quantised(y, None, False)
+    assert float(s) == 1.0 and torch.equal(q, y.float().to(torch.float8_e4m3fn).double())
+    q, s = bo.quantised(y, None, True)
+    assert float(q.abs().max()) == 127
