@@ -57,6 +57,7 @@ bool carry_tc_supported(const palimpsa_problem& p);  // and by the alignment of 
 int launch_carry_tc(const palimpsa_bwd_params* prm, const palimpsa_segments& segs, cudaStream_t stream);
 int carry_tc_status();
 int fwd_wait_status();  // 0, or the code of a bounded wait of the tall-tile forward that gave up
+int ssm_tc_status();    // the same for the state space scan (ssm_tc.cu)
 int bwd_wait_status();  // 0, or the code of a bounded barrier wait of the backward main kernel that gave up
 
 // What a launch of these sizes takes: {1 for the tall-tile kernel, rows of a tile}; {rows, compute warps, group buffers}.

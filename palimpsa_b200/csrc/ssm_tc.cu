@@ -1,8 +1,972 @@
+// Selective state space scan on the 5th-generation tensor cores (tcgen05 + TMEM, TMA): bfloat16, d_k <= 128.
+//
+// Chunks of 128 tokens (formulas in ssm.cuh), d_v in tiles of 64, d_k padded to KP = 64 or 128 by the zeros that TMA fills in.
+//   ssm_walk_kernel   one CTA per sequence, head and tile walks the chunks with the state (or, backwards, its gradient) in
+//                     registers, float32: state <- e^{L_Q} state + (w dt v)^T k, one product per chunk
+//   ssm_out_tc_kernel one CTA per chunk, q/k head and share of its value heads:  S = q k^T once, then per head and tile
+//                     P = S e^{L_i-L_j} dt_j,  o = P v + e^{L_i} q h + D v
+//   ssm_grad_tc_kernel  the same for the gradients; dq and dk of all heads add up in TMEM, and the inner dS = (do v^T) e^.. dt of
+//                     all heads in registers before they meet k and q in one product
+// Operands lie in shared memory as TMA's 128-byte swizzle writes them: [128 tokens][64 columns] boxes, which serve as K-major
+// operand (contraction along the columns) and as MN-major one (contraction along the tokens).  States cross memory as such images
+// too ([KP rows of d_k][64 columns of d_v], bfloat16, two parts hi + lo that give 16 bits), and are fetched by plain bulk copies.
+//
+// Roundings to bfloat16 (products are exact, sums float32 in TMEM): P, dS, e^L do and w dt v as operands of outputs in bfloat16,
+// once, 2^-9 rms of a term; hi of the state where o is made from it.  What ends in float32 -- the states, and q h and k G for the
+// gradients of dt, g and D -- takes both parts of its operand (2^-17), and S and do v^T of the decays' gradients stay float32.
+//
+// Rows of a tile behind a sequence's end are other tokens' or fill; they are zeroed in shared memory, so that whatever they hold
+// never meets a zero weight as NaN.  Every wait is bounded: one that gives up sets g_ssm_status and its CTA's outputs become NaN.
 #include "ssm.cuh"
+#include "tc_common.cuh"
+
 namespace palimpsa {
-bool ssm_tc_supported(const palimpsa_ssm&) { return false; }
-size_t ssm_tc_state_bytes(const palimpsa_ssm&, long long, bool) { return 0; }
-size_t ssm_tc_workspace_bytes(const palimpsa_ssm&, long long) { return 0; }
-int ssm_tc_fwd(const SsmArgs&, bool, cudaStream_t) { return PALIMPSA_E_LAUNCH; }
-int ssm_tc_bwd(const SsmArgs&, cudaStream_t) { return PALIMPSA_E_LAUNCH; }
+
+namespace {
+
+constexpr int Q = SSM_TC_Q;
+constexpr int VT = 64;                 // columns of a tile of d_v
+constexpr int BOX = Q * 128;           // [128 tokens][64 bf16]
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ int g_ssm_status = 0;       // 0, or which kernel's wait gave up: 1 walk, 2 out, 3 gradients
+
+struct TcArgs {
+    SsmArgs s;
+    char* state;             // [chunks][H][tiles][planes][KP][64] bf16
+    char* grad;              // [chunks][H][tiles][2][KP][64]
+    float* part_qk;          // [2][splits][tokens][Hq][K] where heads are split over CTAs
+    int tiles, planes, splits;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     tc::smem_u32(dst)),
+                 "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, unsigned bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(tc::smem_u32(src)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+#define TMEM_OUT8(r) "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+// 8 columns each of three accumulators, or of two.
+__device__ __forceinline__ void tmem_ld8x3(unsigned a0, unsigned a1, unsigned a2, float (&x)[8], float (&y)[8], float (&z)[8]) {
+    unsigned p[8], q[8], r[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%24];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%25];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16,%17,%18,%19,%20,%21,%22,%23}, [%26];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : TMEM_OUT8(p), TMEM_OUT8(q), TMEM_OUT8(r)
+        : "r"(a0), "r"(a1), "r"(a2)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(p[i]), y[i] = __uint_as_float(q[i]), z[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld8x2(unsigned a0, unsigned a1, float (&x)[8], float (&y)[8]) {
+    unsigned p[8], q[8];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : TMEM_OUT8(p), TMEM_OUT8(q)
+        : "r"(a0), "r"(a1)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(p[i]), y[i] = __uint_as_float(q[i]);
+}
+
+// 16-byte chunk `c` (8 columns) of row r of a 128-byte-swizzled tile.
+__device__ __forceinline__ uint4* chunk_at(char* tile, int r, int c) {
+    return reinterpret_cast<uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ void unpack8(uint4 u, float (&x)[8]) {
+    const unsigned r[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(r[i] << 16);
+        x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(tc::pack_bf16(x[0], x[1]), tc::pack_bf16(x[2], x[3]), tc::pack_bf16(x[4], x[5]), tc::pack_bf16(x[6], x[7]));
+}
+// Infinities become the largest finite value, so that a weight beyond float32 does not turn a zero into NaN; NaN stays.
+__device__ __forceinline__ uint4 pack8_finite(const float (&x)[8]) {
+    unsigned r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// Rows len..127 of a box.
+__device__ __forceinline__ void zero_rows(char* box, int len, int tid, int nthr) {
+    for (int i = len * 8 + tid; i < Q * 8; i += nthr) reinterpret_cast<uint4*>(box)[i] = make_uint4(0, 0, 0, 0);
+}
+
+constexpr unsigned A_MN = 1u << 15, B_MN = tc::IDESC_B_MN_MAJOR;
+// D (+)= A B over `steps` of 16 of the contraction.  K-major operands lie in boxes of 64 columns of the contraction; MN-major ones
+// have its rows 128 bytes apart, 64-column boxes of the other dimension BOX apart.
+template <bool AMN, bool BMN>
+__device__ __forceinline__ void product(unsigned d, const char* a, const char* b, int steps, int n, bool acc) {
+    const unsigned id = tc::idesc_bf16(n) | (AMN ? A_MN : 0) | (BMN ? B_MN : 0);
+    const unsigned sa = tc::smem_u32(a), sb = tc::smem_u32(b);
+    for (int k = 0; k < steps; ++k) {
+        const unsigned along = (k >> 2) * BOX + (k & 3) * 32, down = k * 2048;
+        tc::mma(d, AMN ? tc::desc_mn_sw128(sa + down, BOX) : tc::desc_sw128(sa + along),
+                BMN ? tc::desc_mn_sw128(sb + down, BOX) : tc::desc_sw128(sb + along), id, acc || k > 0);
+    }
+}
+
+// A wait that has given up once lets all later ones pass (the outputs are NaN by then).
+struct Waits {
+    bool bad = false;
+    __device__ __forceinline__ void on(unsigned long long* bar, unsigned parity) {
+        if (!tc::mbar_wait(bar, parity, bad ? 64u : tc::SPIN_LIMIT)) bad = true;
+    }
+};
+
+// ---- states, and backwards their gradients, in front of (behind) every chunk ------------------------------------------------------
+constexpr int WALK_THREADS = 128;
+template <int KP>
+constexpr int walk_smem() { return 1024 + (KP / 64) * BOX + BOX + 2 * BOX + 1024; }
+
+template <int KP, bool BACKWARD>
+__global__ void __launch_bounds__(WALK_THREADS) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
+                                                                const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ char raw[];
+    char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
+    char* kt = sm;                          // k (backwards q): KP/64 boxes
+    char* ws = kt + (KP / 64) * BOX;        // w v in two parts; then the state's image in two parts (KP = 64: its rows 64.. of the
+    char* vt = ws + 2 * BOX;                // product are of what lies behind kt, and not read)
+    float* wt = reinterpret_cast<float*>(vt + BOX);
+    __shared__ __align__(8) unsigned long long loaded, made;
+    __shared__ unsigned slot;
+    const SsmArgs& s = g.s;
+    const palimpsa_ssm& a = s.a;
+    const int tid = threadIdx.x, w = tid >> 5, tile = blockIdx.y, nh = blockIdx.x, n = nh / a.H, h = nh - n * a.H, hq = h / (a.H / a.Hq);
+    int first, last;
+    ssm_seq_chunks(s, n, first, last);
+    const int count = last - first;
+    const float* start = BACKWARD ? a.dh_out : a.h0;
+    float* end = BACKWARD ? a.dh0 : a.h_out;
+    const int planes = BACKWARD ? 2 : g.planes;
+    char* images = BACKWARD ? g.grad : g.state;
+    const int k = tid;                      // this thread's row of the state: column k of d_k, 64 columns of d_v
+    const long long at = ((long long)nh * a.V + tile * VT) * a.K + k;
+    float st[VT];
+#pragma unroll
+    for (int v = 0; v < VT; ++v) st[v] = start && k < a.K && tile * VT + v < a.V ? start[at + (long long)v * a.K] : 0.f;
+    if (count > 0) {
+        if (tid == 0) {
+            tc::mbar_init(&loaded);
+            tc::mbar_init(&made);
+            tc::mbar_init_fence();
+            tc::tma_prefetch_map(&kmap);
+            tc::tma_prefetch_map(&vmap);
+        }
+        if (w == 0) tc::tmem_alloc(&slot, 64);
+        tc::fence_before_sync();
+        __syncthreads();
+        tc::fence_after_sync();
+        const unsigned tm = slot;
+        Waits wait;
+        auto load = [&](int i) {  // one thread
+            const SsmChunk ch = ssm_chunk(s, BACKWARD ? last - 1 - i : first + i);
+            tc::mbar_expect_tx(&loaded, (KP / 64 + 1) * BOX);
+#pragma unroll
+            for (int x = 0; x < KP / 64; ++x) tma_load_3d(kt + x * BOX, &kmap, 64 * x, hq, (int)ch.tok, &loaded);
+            tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &loaded);
+        };
+        if (tid == 0) load(0);
+        for (int i = 0; i < count; ++i) {
+            const int c = BACKWARD ? last - 1 - i : first + i;
+            const SsmChunk ch = ssm_chunk(s, c);
+            const long long sc = ((long long)c * a.H + h) * Q;
+            {
+                const float lh = s.lh[sc + tid], ll = s.ll[sc + tid];
+                wt[tid] = BACKWARD ? expf(lh + ll) : expf((s.lh[sc + Q - 1] - lh) + (s.ll[sc + Q - 1] - ll)) * s.dt[sc + tid];
+            }
+            const float decay = expf(s.lh[sc + Q - 1] + s.ll[sc + Q - 1]);
+            if (tid == 0 && i > 0) bulk_store_read();  // the image of the step before has left shared memory
+            wait.on(&loaded, i & 1);
+            __syncthreads();
+            // w v in two parts: row = token, 8 columns a time
+#pragma unroll
+            for (int j = 0; j < Q * 8 / WALK_THREADS; ++j) {
+                const int r = (tid >> 3) + j * (WALK_THREADS / 8), cc = tid & 7;
+                float x[8], hi[8], lo[8];
+                if (r < ch.len) {
+                    unpack8(*chunk_at(vt, r, cc), x);
+                    const float f = wt[r];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = x[e] * f;
+                        hi[e] = __bfloat162float(__float2bfloat16_rn(y));
+                        lo[e] = y - hi[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) hi[e] = lo[e] = 0.f;
+                }
+                *chunk_at(ws, r, cc) = pack8(hi);
+                *chunk_at(ws + BOX, r, cc) = pack8(lo);
+            }
+            if (ch.len < Q)
+#pragma unroll
+                for (int x = 0; x < KP / 64; ++x) zero_rows(kt + x * BOX, ch.len, tid, WALK_THREADS);
+            tc::fence_async_smem();
+            tc::fence_before_sync();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after_sync();
+                product<true, true>(tm, kt, ws, Q / 16, VT, false);
+                product<true, true>(tm, kt, ws + BOX, Q / 16, VT, true);
+                tc::commit(&made);
+            }
+            wait.on(&made, i & 1);
+            tc::fence_after_sync();
+            if (tid == 0 && i + 1 < count) load(i + 1);
+            // the image of the state in front of (behind) this chunk: row k, 64 columns, over the operand that is done with
+            if (k < KP) {
+#pragma unroll
+                for (int cc = 0; cc < 8; ++cc) {
+                    float hi[8], lo[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        hi[e] = __bfloat162float(__float2bfloat16_rn(st[8 * cc + e]));
+                        lo[e] = st[8 * cc + e] - hi[e];
+                    }
+                    *chunk_at(ws, k, cc) = pack8(hi);
+                    if (planes == 2) *chunk_at(ws + KP * 128, k, cc) = pack8(lo);
+                }
+            }
+            tc::fence_async_smem();
+            __syncthreads();
+            if (tid == 0) bulk_store(images + (((long long)c * a.H + h) * g.tiles + tile) * planes * (KP * 128), ws, planes * (KP * 128));
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float r[32];
+                tc::tmem_ld32(tm + ((unsigned)(32 * w) << 16) + 32 * half, r);
+#pragma unroll
+                for (int v = 0; v < 32; ++v) st[32 * half + v] = fmaf(decay, st[32 * half + v], r[v]);
+            }
+            tc::fence_before_sync();
+        }
+        if (wait.bad) {
+            atomicCAS(&g_ssm_status, 0, 1);
+#pragma unroll
+            for (int v = 0; v < VT; ++v) st[v] = __int_as_float(0x7fc00000);
+        }
+        if (tid == 0) bulk_store_done();
+        __syncthreads();
+        if (w == 0) tc::tmem_free(tm, 64);
+    }
+    if (end && k < a.K)
+#pragma unroll
+        for (int v = 0; v < VT; ++v)
+            if (tile * VT + v < a.V) end[at + (long long)v * a.K] = st[v];
+}
+
+// ---- what a head's exponents are made of, in shared memory -------------------------------------------------------------------------
+struct Scalars {
+    float lh[Q], ll[Q], dt[Q], eL[Q], wq[Q];
+    float bl[Q];  // e^{L_m-L_j}, m the last token of j's block of 32: what column j brings to rows of later blocks
+};
+__device__ __forceinline__ void load_scalars(Scalars& x, const SsmArgs& s, int c, int h, int tid) {
+    if (tid < Q) {
+        const long long at = ((long long)c * s.a.H + h) * Q, m = at + (tid | 31);
+        const float lh = s.lh[at + tid], ll = s.ll[at + tid];
+        x.lh[tid] = lh, x.ll[tid] = ll, x.dt[tid] = s.dt[at + tid];
+        x.eL[tid] = expf(lh + ll);
+        x.wq[tid] = expf((s.lh[at + Q - 1] - lh) + (s.ll[at + Q - 1] - ll));
+        x.bl[tid] = expf((s.lh[m] - lh) + (s.ll[m] - ll));
+    }
+}
+// 32 values of row r, columns 32 cb .., into an operand of two boxes.
+__device__ __forceinline__ void st_block(char* tile, int r, int cb, const float (&p)[32]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[8 * q + e];
+        *chunk_at(tile + (cb >> 1) * BOX, r, (cb & 1) * 4 + q) = pack8_finite(x);
+    }
+}
+__device__ __forceinline__ void zero_tile(char* tile, int bytes, int tid, int nthr) {
+    for (int i = tid; i < bytes / 16; i += nthr) reinterpret_cast<uint4*>(tile)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---- outputs --------------------------------------------------------------------------------------------------------------------------
+constexpr int THREADS = 256;  // 8 warps: rows 32 (w % 4) .., column half w / 4
+template <int KP>
+constexpr int out_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * 2 * BOX + 2 * BOX + 2 * KP * 128 + 2 * (int)sizeof(Scalars); }
+
+template <int KP>
+__global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, const __grid_constant__ CUtensorMap qmap,
+                                                             const __grid_constant__ CUtensorMap kmap,
+                                                             const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ char raw[];
+    char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
+    char* qt = sm;
+    char* kt = qt + (KP / 64) * BOX;
+    char* P = kt + (KP / 64) * BOX;        // two operands of two boxes
+    char* vt = P + 4 * BOX;                // two tiles of v
+    char* ht = vt + 2 * BOX;               // two states (hi)
+    Scalars* sc = reinterpret_cast<Scalars*>(ht + 2 * KP * 128);
+    __shared__ __align__(8) unsigned long long qk_loaded, loaded[2], s_made, made[2];
+    __shared__ unsigned slot;
+    const SsmArgs& s = g.s;
+    const palimpsa_ssm& a = s.a;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, c = blockIdx.x, hq = blockIdx.y, rep = a.H / a.Hq;
+    const SsmChunk ch = ssm_chunk(s, c);
+    if (ch.len == 0) return;
+    // this CTA's share of the heads and tiles that read hq
+    const int all = rep * g.tiles, per = (all + g.splits - 1) / g.splits, j0 = blockIdx.z * per, j1 = min(all, j0 + per);
+    if (j0 >= j1) return;
+    if (tid == 0) {
+        tc::mbar_init(&qk_loaded);
+        tc::mbar_init(&s_made);
+        for (int b = 0; b < 2; ++b) tc::mbar_init(&loaded[b]), tc::mbar_init(&made[b]);
+        tc::mbar_init_fence();
+    }
+    if (w == 0) tc::tmem_alloc(&slot, 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const unsigned tm = slot, tS = tm, tY = tm + 128, tU = tm + 256;  // S 128; two Y and two U of 64 columns
+    auto load = [&](int j) {  // one thread
+        const int b = (j - j0) & 1, h = hq * rep + j / g.tiles, tile = j % g.tiles;
+        tc::mbar_expect_tx(&loaded[b], BOX + KP * 128);
+        tma_load_3d(vt + b * BOX, &vmap, tile * VT, h, (int)ch.tok, &loaded[b]);
+        bulk_load(ht + b * KP * 128, g.state + (((long long)c * a.H + h) * g.tiles + tile) * g.planes * (KP * 128), KP * 128, &loaded[b]);
+    };
+    if (tid == 0) {
+        tc::mbar_expect_tx(&qk_loaded, 2 * (KP / 64) * BOX);
+#pragma unroll
+        for (int x = 0; x < KP / 64; ++x) {
+            tma_load_3d(qt + x * BOX, &qmap, 64 * x, hq, (int)ch.tok, &qk_loaded);
+            tma_load_3d(kt + x * BOX, &kmap, 64 * x, hq, (int)ch.tok, &qk_loaded);
+        }
+        load(j0);
+        if (j0 + 1 < j1) load(j0 + 1);
+    }
+    Waits wait;
+    zero_tile(P, 4 * BOX, tid, THREADS);  // the blocks above the diagonal stay zero
+    wait.on(&qk_loaded, 0);
+    __syncthreads();
+    if (ch.len < Q) {
+#pragma unroll
+        for (int x = 0; x < KP / 64; ++x) zero_rows(qt + x * BOX, ch.len, tid, THREADS), zero_rows(kt + x * BOX, ch.len, tid, THREADS);
+        tc::fence_async_smem();
+        __syncthreads();
+    }
+    if (tid == 0) {
+        product<false, false>(tS, qt, kt, KP / 16, Q, false);
+        tc::commit(&s_made);
+    }
+    wait.on(&s_made, 0);
+    tc::fence_after_sync();
+    const int rw = w & 3, half = w >> 2, r = 32 * rw + lane;
+    const unsigned lanes = (unsigned)(32 * rw) << 16;
+    auto finish = [&](int j) {  // o of head and tile j
+        const int b = (j - j0) & 1, h = hq * rep + j / g.tiles, v0 = (j % g.tiles) * VT;
+        wait.on(&made[b], ((j - j0) >> 1) & 1);
+        tc::fence_after_sync();
+        const float e = sc[b].eL[r], D = a.D ? a.D[h] : 0.f;
+        char* x = vt + b * BOX;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int cc = 4 * half + q;
+            float y[8], u[8], v[8];
+            tmem_ld8x2(tY + lanes + 64 * b + 8 * cc, tU + lanes + 64 * b + 8 * cc, y, u);
+            unpack8(*chunk_at(x, r, cc), v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = fmaf(e, u[i], fmaf(D, v[i], y[i]));
+                if (wait.bad) y[i] = __int_as_float(0x7fc00000);
+            }
+            *chunk_at(x, r, cc) = pack8(y);
+        }
+        tc::fence_before_sync();
+        __syncthreads();
+        char* o = static_cast<char*>(a.o) + ((ch.tok * a.H + h) * a.V + v0) * 2;
+#pragma unroll
+        for (int i = 0; i < Q * 8 / THREADS; ++i) {
+            const int row = (tid >> 3) + i * (THREADS / 8), cc = tid & 7;
+            if (row < ch.len && v0 + 8 * cc < a.V) *reinterpret_cast<uint4*>(o + ((long long)row * a.H * a.V + 8 * cc) * 2) = *chunk_at(x, row, cc);
+        }
+        tc::fence_async_smem();
+        __syncthreads();
+        if (tid == 0 && j + 2 < j1) load(j + 2);
+    };
+    for (int j = j0; j < j1; ++j) {
+        const int n = j - j0, b = n & 1, h = hq * rep + j / g.tiles;
+        load_scalars(sc[b], s, c, h, tid);
+        wait.on(&loaded[b], (n >> 1) & 1);
+        __syncthreads();
+        if (ch.len < Q) {
+            zero_rows(vt + b * BOX, ch.len, tid, THREADS);
+            tc::fence_async_smem();
+        }
+        if (tid == 0) {
+            tc::fence_after_sync();
+            product<false, true>(tU + 64 * b, qt, ht + b * KP * 128, KP / 16, VT, false);
+        }
+        const Scalars& x = sc[b];
+        char* p = P + b * 2 * BOX;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int cb = 2 * half + k;
+            if (cb > rw) break;
+            float t[32];
+            tc::tmem_ld32(tS + lanes + 32 * cb, t);
+            const float lh = x.lh[r], ll = x.ll[r];
+            if (cb < rw) {
+                const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) t[i] *= ai * (x.bl[32 * cb + i] * x.dt[32 * cb + i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float d = (lh - x.lh[32 * cb + i]) + (ll - x.ll[32 * cb + i]);
+                    t[i] = i <= lane ? t[i] * ex2(d * LOG2E) * x.dt[32 * cb + i] : 0.f;
+                }
+            }
+            st_block(p, r, cb, t);
+        }
+        tc::fence_async_smem();
+        tc::fence_before_sync();
+        __syncthreads();
+        if (tid == 0) {
+            tc::fence_after_sync();
+            product<false, true>(tY + 64 * b, p, vt + b * BOX, Q / 16, VT, false);
+            tc::commit(&made[b]);
+        }
+        if (n > 0) finish(j - 1);
+    }
+    finish(j1 - 1);
+    if (wait.bad && tid == 0) atomicCAS(&g_ssm_status, 0, 2);
+    __syncthreads();
+    if (w == 0) tc::tmem_free(tm, 512);
+}
+
+// ---- gradients ------------------------------------------------------------------------------------------------------------------------
+struct GradSums {            // of a head, over its tiles
+    float row[2][Q];         // sum_j M_ij over the columns of earlier blocks
+    float col[4][Q];         // sum over the rows of block w of P_ij (do_i.v_j): M_ij / dt_j
+    float z[Q];              // sum_{i>=t>j} M_ij inside t's own block
+    float A[2][Q], B[2][Q];  // do_i.(h q_i), v_j.(G k_j), by halves of d_v
+    float dot[8], diag[4];   // <h, G>; do_i.v_i
+    float cross[4][4], at[4], bt[4], pg[4], pb[4];
+};
+template <int KP>
+constexpr int grad_smem() {
+    return 1024 + 2 * (KP / 64) * BOX + 2 * BOX + 2 * BOX + 4 * KP * 128 + (int)sizeof(Scalars) + (int)sizeof(GradSums);
+}
+
+template <int KP>
+__global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g, const __grid_constant__ CUtensorMap qmap,
+                                                              const __grid_constant__ CUtensorMap kmap,
+                                                              const __grid_constant__ CUtensorMap vmap,
+                                                              const __grid_constant__ CUtensorMap dmap) {
+    extern __shared__ char raw[];
+    char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
+    char* qt = sm;
+    char* kt = qt + (KP / 64) * BOX;
+    char* P = kt + (KP / 64) * BOX;        // P_ij; where it is done with, dv on its way out; at the end dS
+    char* vt = P + 2 * BOX;
+    char* dy = vt + BOX;
+    char* ht = dy + BOX;                   // h hi, lo
+    char* gt = ht + 2 * KP * 128;          // G hi, lo
+    Scalars& x = *reinterpret_cast<Scalars*>(gt + 2 * KP * 128);
+    GradSums& sums = *reinterpret_cast<GradSums*>(&x + 1);
+    __shared__ __align__(8) unsigned long long qk_loaded, loaded, inner, pv, outer;
+    __shared__ unsigned slot;
+    const SsmArgs& s = g.s;
+    const palimpsa_ssm& a = s.a;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, c = blockIdx.x, hq = blockIdx.y, rep = a.H / a.Hq;
+    const SsmChunk ch = ssm_chunk(s, c);
+    if (ch.len == 0) return;
+    const int per = (rep + g.splits - 1) / g.splits, h0 = hq * rep + blockIdx.z * per, h1 = min((hq + 1) * rep, h0 + per);
+    if (h0 >= h1) return;                  // (the launch leaves no share empty)
+    if (tid == 0) {
+        for (unsigned long long* b : {&qk_loaded, &loaded, &inner, &pv, &outer}) tc::mbar_init(b);
+        tc::mbar_init_fence();
+    }
+    if (w == 0) tc::tmem_alloc(&slot, 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    // do v^T, then P^T do over it; q h and k G; dq and dk
+    const unsigned tm = slot, tD = tm, tU = tm + 128, tG = tm + 192, tQ = tm + 256, tK = tm + 256 + KP;
+    auto load = [&](int h, int tile) {  // one thread
+        tc::mbar_expect_tx(&loaded, 2 * BOX + 4 * KP * 128);
+        tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &loaded);
+        tma_load_3d(dy, &dmap, tile * VT, h, (int)ch.tok, &loaded);
+        const long long at = (((long long)c * a.H + h) * g.tiles + tile) * 2 * (KP * 128);
+        bulk_load(ht, g.state + at, 2 * KP * 128, &loaded);
+        bulk_load(gt, g.grad + at, 2 * KP * 128, &loaded);
+    };
+    if (tid == 0) {
+        tc::mbar_expect_tx(&qk_loaded, 2 * (KP / 64) * BOX);
+#pragma unroll
+        for (int b = 0; b < KP / 64; ++b) {
+            tma_load_3d(qt + b * BOX, &qmap, 64 * b, hq, (int)ch.tok, &qk_loaded);
+            tma_load_3d(kt + b * BOX, &kmap, 64 * b, hq, (int)ch.tok, &qk_loaded);
+        }
+        load(h0, 0);
+    }
+    Waits wait;
+    zero_tile(P, 2 * BOX, tid, THREADS);
+    wait.on(&qk_loaded, 0);
+    __syncthreads();
+    if (ch.len < Q)
+#pragma unroll
+        for (int b = 0; b < KP / 64; ++b) zero_rows(qt + b * BOX, ch.len, tid, THREADS), zero_rows(kt + b * BOX, ch.len, tid, THREADS);
+    tc::fence_async_smem();
+    __syncthreads();
+    if (tid == 0) {
+        product<false, false>(tD, qt, kt, KP / 16, Q, false);
+        tc::commit(&inner);
+    }
+    const int rw = w & 3, half = w >> 2, r = 32 * rw + lane;
+    const unsigned lanes = (unsigned)(32 * rw) << 16;
+    float S[2][32], dS[2][32];  // of blocks 2 half and 2 half + 1, where they are not above the diagonal
+    wait.on(&inner, 0);
+    tc::fence_after_sync();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        tc::tmem_ld32(tD + lanes + 32 * (2 * half + k), S[k]);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) dS[k][i] = 0.f;
+    }
+    tc::fence_before_sync();
+    int step = 0;
+    for (int h = h0; h < h1; ++h) {
+        for (int tile = 0; tile < g.tiles; ++tile, ++step) {
+            if (tile == 0) load_scalars(x, s, c, h, tid);
+            wait.on(&loaded, step & 1);
+            __syncthreads();
+            if (ch.len < Q) {
+                zero_rows(vt, ch.len, tid, THREADS);
+                zero_rows(dy, ch.len, tid, THREADS);
+                tc::fence_async_smem();
+                __syncthreads();
+            }
+            if (tid == 0) {
+                tc::fence_after_sync();
+                product<false, false>(tD, dy, vt, VT / 16, Q, false);
+                tc::commit(&inner);
+                product<false, true>(tU, qt, ht, KP / 16, VT, false);
+                product<false, true>(tU, qt, ht + KP * 128, KP / 16, VT, true);
+                product<false, true>(tG, kt, gt, KP / 16, VT, false);
+                product<false, true>(tG, kt, gt + KP * 128, KP / 16, VT, true);
+            }
+            auto put = [tile](float& to, float y) { to = tile ? to + y : y; };
+            {   // <h, G>
+                float d = 0.f;
+                for (int i = tid; i < KP * 8; i += THREADS) {
+                    float p[8], q[8], u[8], v[8];
+                    unpack8(reinterpret_cast<const uint4*>(ht)[i], p);
+                    unpack8(reinterpret_cast<const uint4*>(ht + KP * 128)[i], q);
+                    unpack8(reinterpret_cast<const uint4*>(gt)[i], u);
+                    unpack8(reinterpret_cast<const uint4*>(gt + KP * 128)[i], v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) d = fmaf(p[e] + q[e], u[e] + v[e], d);
+                }
+                d = warp_add(d);
+                if (lane == 0) put(sums.dot[w], d);
+            }
+            wait.on(&inner, (step + 1) & 1);
+            tc::fence_after_sync();
+            float early = 0.f;
+            const float lh = x.lh[r], ll = x.ll[r];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int cb = 2 * half + k;
+                if (cb > rw) break;
+                float t[32], p[32];
+                tc::tmem_ld32(tD + lanes + 32 * cb, t);
+                if (cb < rw) {
+                    const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float dec = ai * x.bl[32 * cb + i], dt = x.dt[32 * cb + i], q = t[i] * dec;
+                        p[i] = S[k][i] * dec;
+                        t[i] = q * S[k][i];
+                        dS[k][i] = fmaf(q, dt, dS[k][i]);
+                        early = fmaf(t[i], dt, early);
+                    }
+                    st_block(P, r, cb, p);
+                } else {
+                    float diag = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float d = (lh - x.lh[32 * cb + i]) + (ll - x.ll[32 * cb + i]);
+                        const float dec = i <= lane ? ex2(d * LOG2E) : 0.f, q = i <= lane ? t[i] * dec : 0.f;
+                        if (i == lane) diag = t[i];
+                        p[i] = i <= lane ? S[k][i] * dec : 0.f;
+                        t[i] = q * S[k][i];
+                        dS[k][i] = fmaf(q, x.dt[32 * cb + i], dS[k][i]);
+                    }
+                    st_block(P, r, cb, p);
+                    // row i brings sum_{j<t} M_ij to the borders t <= i
+                    float run = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        p[i] = i <= lane ? run : 0.f;
+                        run = fmaf(t[i], x.dt[32 * cb + i], run);
+                    }
+                    xreduce<32, 32>(p, lane);
+                    put(sums.z[32 * cb + xreduce_index<32, 32>(lane)], p[0]);
+                    diag = warp_add(diag);
+                    if (lane == 0) put(sums.diag[cb], diag);
+                }
+                xreduce<32, 32>(t, lane);
+                put(sums.col[rw][32 * cb + xreduce_index<32, 32>(lane)], t[0]);
+            }
+            put(sums.row[half][r], early);
+            tc::fence_async_smem();
+            tc::fence_before_sync();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after_sync();
+                product<true, true>(tD, P, dy, Q / 16, VT, false);
+                tc::commit(&pv);
+            }
+            wait.on(&pv, step & 1);
+            tc::fence_after_sync();
+            {   // row r of all three, 32 columns: dv, and what do and v become as operands of dq and dk
+                float A = 0.f, B = 0.f;
+                const float dt = x.dt[r], wq = x.wq[r], eL = x.eL[r], wd = wq * dt, D = a.D ? a.D[h] : 0.f;
+                char* out = P + (r < 96 ? (32 + r) * 128 : BOX + r * 128);  // rows of P that every head writes anew
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int cc = 4 * half + q;
+                    float u1[8], u2[8], pd[8], v[8], d[8];
+                    tmem_ld8x3(tU + lanes + 8 * cc, tG + lanes + 8 * cc, tD + lanes + 8 * cc, u1, u2, pd);
+                    unpack8(*chunk_at(vt, r, cc), v);
+                    unpack8(*chunk_at(dy, r, cc), d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        A = fmaf(d[i], u1[i], A);
+                        B = fmaf(v[i], u2[i], B);
+                        pd[i] = fmaf(dt, fmaf(wq, u2[i], pd[i]), D * d[i]);
+                        if (wait.bad) pd[i] = __int_as_float(0x7fc00000);
+                        v[i] *= wd;
+                        d[i] *= eL;
+                    }
+                    reinterpret_cast<uint4*>(out)[cc ^ (r & 7)] = pack8(pd);
+                    *chunk_at(vt, r, cc) = pack8(v);
+                    *chunk_at(dy, r, cc) = pack8(d);
+                }
+                put(sums.A[half][r], A);
+                put(sums.B[half][r], B);
+            }
+            tc::fence_async_smem();
+            tc::fence_before_sync();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after_sync();
+                product<false, false>(tQ, dy, ht, VT / 16, KP, step > 0);
+                product<false, false>(tK, vt, gt, VT / 16, KP, step > 0);
+                tc::commit(&outer);
+            }
+            const int v0 = tile * VT;
+            char* dv = static_cast<char*>(a.dv) + ((ch.tok * a.H + h) * a.V + v0) * 2;
+#pragma unroll
+            for (int i = 0; i < Q * 8 / THREADS; ++i) {
+                const int row = (tid >> 3) + i * (THREADS / 8), cc = tid & 7;
+                const char* from = P + (row < 96 ? (32 + row) * 128 : BOX + row * 128);
+                if (row < ch.len && v0 + 8 * cc < a.V)
+                    *reinterpret_cast<uint4*>(dv + ((long long)row * a.H * a.V + 8 * cc) * 2) = reinterpret_cast<const uint4*>(from)[cc ^ (row & 7)];
+            }
+            if (tile + 1 == g.tiles) {  // the head's scalars: thread t of the first 128 has token t, of block b
+                const int t = tid, b = w;
+                float ta = 0.f, tb = 0.f, late = 0.f, own = 0.f, direct = 0.f, dt = 0.f;
+                if (tid < Q) {
+                    dt = x.dt[t];
+                    ta = x.eL[t] * (sums.A[0][t] + sums.A[1][t]);
+                    own = x.wq[t] * (sums.B[0][t] + sums.B[1][t]);
+                    tb = dt * own;
+                    direct = sums.col[b][t];
+                    for (int k = b + 1; k < 4; ++k) {
+                        const float y = sums.col[k][t];
+                        direct += y;
+                        late = fmaf(y, dt, late);
+                        const float total = warp_add(y * dt);
+                        if (lane == 0) sums.cross[k][b] = total;
+                    }
+                    const float at = warp_add(ta), bt = warp_add(tb);
+                    if (lane == 0) sums.at[b] = at, sums.bt[b] = bt;
+                }
+                __syncthreads();
+                if (tid < Q) {
+                    float suf = sums.row[0][t] + sums.row[1][t] + ta, pre = late + tb;
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) {
+                        const float y = __shfl_down_sync(0xffffffffu, suf, d), u = __shfl_up_sync(0xffffffffu, pre, d);
+                        if (lane + d < 32) suf += y;
+                        if (lane >= d) pre += u;
+                    }
+                    pre = __shfl_up_sync(0xffffffffu, pre, 1);
+                    float dlf = sums.z[t] + suf + (lane ? pre : 0.f), hG = 0.f;
+                    for (int k = b + 1; k < 4; ++k) dlf += sums.at[k];
+                    for (int k = 0; k < b; ++k) dlf += sums.bt[k];
+                    for (int k = b + 1; k < 4; ++k)
+                        for (int i = 0; i < b; ++i) dlf += sums.cross[k][i];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) hG += sums.dot[k];
+                    dlf = fmaf(x.eL[Q - 1], hG, dlf);
+                    float ddt = direct + own - a.g[h] * dlf;
+                    float pg = 0.f, pb = 0.f;
+                    if (wait.bad) ddt = dlf = __int_as_float(0x7fc00000);
+                    if (t < ch.len) {
+                        const long long at = (ch.tok + t) * a.H + h;
+                        const float u = ld_any(a.gt, at, a.gt_dtype) + (a.gt_bias ? a.gt_bias[h] : 0.f);
+                        ddt *= ssm_ddt(u, (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0);
+                        st1(a.dgt, at, ddt, a.gt_dtype);
+                        pg = -dt * dlf, pb = ddt;
+                    }
+                    pg = warp_add(pg), pb = warp_add(pb);
+                    if (lane == 0) sums.pg[b] = pg, sums.pb[b] = pb;
+                }
+                __syncthreads();
+                if (tid == 0) {
+                    const long long n = (long long)s.chunks * a.H, at = (long long)c * a.H + h;
+                    s.part[at] = sums.pg[0] + sums.pg[1] + sums.pg[2] + sums.pg[3];
+                    s.part[n + at] = sums.pb[0] + sums.pb[1] + sums.pb[2] + sums.pb[3];
+                    s.part[2 * n + at] = sums.diag[0] + sums.diag[1] + sums.diag[2] + sums.diag[3];
+                }
+            }
+            wait.on(&outer, step & 1);
+            tc::fence_after_sync();
+            tc::fence_async_smem();
+            __syncthreads();  // P, the scalars and the sums may be written again
+            if (tid == 0) {
+                if (tile + 1 < g.tiles) load(h, tile + 1);
+                else if (h + 1 < h1) load(h + 1, 0);
+            }
+        }
+    }
+    // dq += dS k, dk += dS^T q
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (2 * half + k <= rw) st_block(P, r, 2 * half + k, dS[k]);
+    tc::fence_async_smem();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (tid == 0) {
+        tc::fence_after_sync();
+        product<false, true>(tQ, P, kt, Q / 16, KP, true);
+        product<true, true>(tK, P, qt, Q / 16, KP, true);
+        tc::commit(&outer);
+    }
+    wait.on(&outer, step & 1);
+    tc::fence_after_sync();
+    // dq by the first four warps, dk by the others: a row each, 8 columns a time
+    {
+        const unsigned from = (half ? tK : tQ) + lanes;
+        const long long row = (ch.tok + r) * a.Hq + hq;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(half ? a.dk : a.dq) + row * a.K;
+        float* part = g.splits > 1 ? g.part_qk + (((long long)half * g.splits + blockIdx.z) * a.total_tokens * a.Hq + row) * a.K : nullptr;
+#pragma unroll 1
+        for (int k0 = 0; k0 < KP; k0 += 16) {
+            float y[8], z[8];
+            tmem_ld8x2(from + k0, from + k0 + 8, y, z);
+            if (wait.bad) y[0] = z[0] = __int_as_float(0x7fc00000);
+            if (r < ch.len) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int k = k0 + 8 * p;
+                    float(&v)[8] = p ? z : y;
+                    if (k < a.K) {
+                        if (part) {
+                            *reinterpret_cast<float4*>(part + k) = make_float4(v[0], v[1], v[2], v[3]);
+                            *reinterpret_cast<float4*>(part + k + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                        } else {
+                            *reinterpret_cast<uint4*>(out + k) = pack8(v);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if (wait.bad && tid == 0) atomicCAS(&g_ssm_status, 0, 3);
+    tc::fence_before_sync();
+    __syncthreads();
+    if (w == 0) tc::tmem_free(tm, 512);
+}
+
+// dq and dk where heads were split over CTAs: the shares in their order.  Rows outside of every sequence have none.
+__global__ void __launch_bounds__(256) ssm_join_kernel(const TcArgs g) {
+    const palimpsa_ssm& a = g.s.a;
+    const long long n = a.total_tokens * a.Hq * a.K / 8, i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    if (a.cu_seqlens) {
+        const long long t = i * 8 / ((long long)a.Hq * a.K);
+        if (t < clamped_offset(a.cu_seqlens, 0, a.total_tokens) || t >= clamped_offset(a.cu_seqlens, a.num_seqs, a.total_tokens)) return;
+    }
+    const float* p = g.part_qk + (long long)blockIdx.y * g.splits * n * 8 + i * 8;
+    float x[8] = {};
+    for (int k = 0; k < g.splits; ++k) {
+        const float4 y = reinterpret_cast<const float4*>(p + k * n * 8)[0], z = reinterpret_cast<const float4*>(p + k * n * 8)[1];
+        x[0] += y.x, x[1] += y.y, x[2] += y.z, x[3] += y.w, x[4] += z.x, x[5] += z.y, x[6] += z.z, x[7] += z.w;
+    }
+    reinterpret_cast<uint4*>(blockIdx.y ? a.dk : a.dq)[i] = pack8(x);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------------
+// [tokens][heads][cols] of bf16, token rows `stride` elements apart, boxes of 128 tokens x 64 columns of one head.
+bool token_map(CUtensorMap* map, const void* base, long long tokens, int heads, int cols, long long stride) {
+    typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static encode_fn encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<encode_fn>(fn);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, Q}, each[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+int padded(int K) { return K <= 64 ? 64 : 128; }
+int tiles_of(const palimpsa_ssm& a) { return (a.V + VT - 1) / VT; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int launched() { return cudaGetLastError() == cudaSuccess ? PALIMPSA_OK : PALIMPSA_E_LAUNCH; }
+
+// Into how many shares a chunk's heads (times tiles where `tiles` of them may be parted) go: whole waves of CTAs times what one
+// takes, with `fixed` steps for what a CTA does once.
+int shares(long long ctas, int steps, double fixed) {
+    int best = 1;
+    double least = 1e30;
+    for (int n = 1; n <= steps; ++n) {
+        const int per = (steps + n - 1) / n;
+        if ((steps + per - 1) / per != n) continue;  // the same shares as a smaller n, some empty
+        const double cost = (double)((ctas * n + B200_SMS - 1) / B200_SMS) * (per + fixed);
+        if (cost < least * 0.97) least = cost, best = n;
+    }
+    return best;
+}
+int grad_shares(const palimpsa_ssm& a, long long chunks) { return shares(chunks * a.Hq, a.H / a.Hq, 1.5 / tiles_of(a)); }
+
+TcArgs tc_args(const SsmArgs& s, bool training) {
+    TcArgs g{};
+    g.s = s;
+    g.state = reinterpret_cast<char*>(s.state);
+    g.grad = reinterpret_cast<char*>(s.grad);
+    g.tiles = tiles_of(s.a);
+    g.planes = training ? 2 : 1;
+    return g;
+}
+size_t image_bytes(const palimpsa_ssm& a, long long chunks) { return (size_t)chunks * a.H * tiles_of(a) * padded(a.K) * 128; }
+
+}  // namespace
+
+bool ssm_tc_supported(const palimpsa_ssm& a) {
+    return a.io_dtype == PALIMPSA_BF16 && a.K % 8 == 0 && a.K <= 128 && a.V % 8 == 0 && a.q_stride % 8 == 0 && a.k_stride % 8 == 0 &&
+           a.v_stride % 8 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && a.Hq <= 65535;
+}
+size_t ssm_tc_state_bytes(const palimpsa_ssm& a, long long chunks, bool training) { return image_bytes(a, chunks) * (training ? 2 : 1); }
+size_t ssm_tc_workspace_bytes(const palimpsa_ssm& a, long long chunks) {
+    const int n = grad_shares(a, chunks);
+    return image_bytes(a, chunks) * 2 + (n > 1 ? (size_t)2 * n * a.total_tokens * a.Hq * a.K * 4 : 0);
+}
+
+template <int KP, bool BACKWARD>
+static int launch_walk(const TcArgs& g, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
+    const palimpsa_ssm& a = g.s.a;
+    if (!allow_smem<ssm_walk_kernel<KP, BACKWARD>>(walk_smem<KP>())) return PALIMPSA_E_LAUNCH;
+    ssm_walk_kernel<KP, BACKWARD><<<dim3(a.num_seqs * a.H, g.tiles), WALK_THREADS, walk_smem<KP>(), st>>>(g, kmap, vmap);
+    return launched();
+}
+
+int ssm_tc_fwd(const SsmArgs& s, bool training, cudaStream_t st) {
+    const palimpsa_ssm& a = s.a;
+    if (!aligned16(a.o)) return PALIMPSA_E_ALIGN;
+    TcArgs g = tc_args(s, training);
+    CUtensorMap q{}, k{}, v{};
+    if (a.total_tokens > 0 && (!token_map(&q, a.q, a.total_tokens, a.Hq, a.K, a.q_stride) ||
+                               !token_map(&k, a.k, a.total_tokens, a.Hq, a.K, a.k_stride) ||
+                               !token_map(&v, a.v, a.total_tokens, a.H, a.V, a.v_stride)))
+        return PALIMPSA_E_LAUNCH;
+    const bool wide = padded(a.K) == 128;
+    if (a.num_seqs > 0)
+        if (int rc = wide ? launch_walk<128, false>(g, k, v, st) : launch_walk<64, false>(g, k, v, st)) return rc;
+    if (s.chunks == 0) return PALIMPSA_OK;
+    g.splits = shares((long long)s.chunks * a.Hq, a.H / a.Hq * g.tiles, 2.);
+    const dim3 grid(s.chunks, a.Hq, g.splits);
+    if (wide) {
+        if (!allow_smem<ssm_out_tc_kernel<128>>(out_smem<128>())) return PALIMPSA_E_LAUNCH;
+        ssm_out_tc_kernel<128><<<grid, THREADS, out_smem<128>(), st>>>(g, q, k, v);
+    } else {
+        if (!allow_smem<ssm_out_tc_kernel<64>>(out_smem<64>())) return PALIMPSA_E_LAUNCH;
+        ssm_out_tc_kernel<64><<<grid, THREADS, out_smem<64>(), st>>>(g, q, k, v);
+    }
+    return launched();
+}
+
+int ssm_tc_bwd(const SsmArgs& s, cudaStream_t st) {
+    const palimpsa_ssm& a = s.a;
+    for (const void* p : {a.d_o, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
+        if (!aligned16(p)) return PALIMPSA_E_ALIGN;
+    TcArgs g = tc_args(s, true);
+    CUtensorMap q{}, k{}, v{}, d{};
+    if (a.total_tokens > 0 && (!token_map(&q, a.q, a.total_tokens, a.Hq, a.K, a.q_stride) ||
+                               !token_map(&k, a.k, a.total_tokens, a.Hq, a.K, a.k_stride) ||
+                               !token_map(&v, a.v, a.total_tokens, a.H, a.V, a.v_stride) ||
+                               !token_map(&d, a.d_o, a.total_tokens, a.H, a.V, (long long)a.H * a.V)))
+        return PALIMPSA_E_LAUNCH;
+    const bool wide = padded(a.K) == 128;
+    if (a.num_seqs > 0)
+        if (int rc = wide ? launch_walk<128, true>(g, q, d, st) : launch_walk<64, true>(g, q, d, st)) return rc;
+    if (s.chunks == 0) return PALIMPSA_OK;
+    g.splits = grad_shares(a, s.chunks);
+    g.part_qk = reinterpret_cast<float*>(g.grad + image_bytes(a, s.chunks) * 2);
+    const dim3 grid(s.chunks, a.Hq, g.splits);
+    if (wide) {
+        if (!allow_smem<ssm_grad_tc_kernel<128>>(grad_smem<128>())) return PALIMPSA_E_LAUNCH;
+        ssm_grad_tc_kernel<128><<<grid, THREADS, grad_smem<128>(), st>>>(g, q, k, v, d);
+    } else {
+        if (!allow_smem<ssm_grad_tc_kernel<64>>(grad_smem<64>())) return PALIMPSA_E_LAUNCH;
+        ssm_grad_tc_kernel<64><<<grid, THREADS, grad_smem<64>(), st>>>(g, q, k, v, d);
+    }
+    if (int rc = launched()) return rc;
+    if (g.splits > 1) {
+        const long long n = a.total_tokens * a.Hq * a.K / 8;
+        ssm_join_kernel<<<dim3((unsigned)((n + 255) / 256), 2), 256, 0, st>>>(g);
+    }
+    return launched();
+}
+
+int ssm_tc_status() {
+    int x = 0;
+    if (cudaMemcpyFromSymbol(&x, g_ssm_status, sizeof(int)) != cudaSuccess) return -1;
+    if (x) {
+        const int zero = 0;
+        if (cudaMemcpyToSymbol(g_ssm_status, &zero, sizeof(int)) != cudaSuccess) return -1;
+    }
+    return x;
+}
+
 }  // namespace palimpsa

@@ -154,15 +154,20 @@ def test_rows_apart_are_read_in_place_and_copied_where_they_must_be():
             row = torch.cat([wide, wide.new_zeros(2, T, pad)], -1) if pad else wide
             v, k, q, _ = row.split([H * V, Hq * K, Hq * K, pad], -1)
             o = chunk_ssm(q.unflatten(-1, (Hq, K)), k.unflatten(-1, (Hq, K)), v.unflatten(-1, (H, V)), x["gt"], x["g"], gt_softplus=True)
-            assert torch.allclose(o.float(), base.float(), atol=2e-2 if dtype == torch.bfloat16 else 1e-5, rtol=2e-2 if pad == 1 else 0)
-            if pad != 1:
+            if pad != 1 or dtype == torch.float32:
                 assert torch.equal(o, base)
+            else:    # CUDA cores here, tensor cores there: each within its bound of the recurrence, see the top
+                mag = bo.ssm(d["q"], d["k"], d["v"], d["gt"], d["g"], softplus=True, magnitude=True)["o"]
+                bound = 3.1 * 2.0 ** -8 * mag + 2 * 2.0 ** -8 * base.cpu().double().abs() * (1 + 2.0 ** -6)
+                assert ((o.double() - base.double()).abs().cpu() <= bound).all()
         heads_first = x["v"].transpose(1, 2).contiguous().transpose(1, 2)
         assert torch.equal(chunk_ssm(x["q"], x["k"], heads_first, x["gt"], x["g"], gt_softplus=True), base)
         assert torch.equal(chunk_ssm(x["q"][:, ::2], x["k"][:, ::2], x["v"][:, ::2], x["gt"][:, ::2], x["g"]),
                            chunk_ssm(*[x[n][:, ::2].contiguous() for n in ("q", "k", "v", "gt")], x["g"]))
-        one = x["q"][:, :1].expand(-1, T, -1, -1)      # stride 0
-        assert torch.equal(chunk_ssm(one, one, x["v"], x["gt"], x["g"]), chunk_ssm(one.contiguous(), one.contiguous(), x["v"], x["gt"], x["g"]))
+        one = x["q"][:, :1].expand(-1, T, -1, -1)      # stride 0; steps below zero let the state grow past float32: compare the bits
+        bits = lambda y: y.view(torch.int16 if dtype == torch.bfloat16 else torch.int32)
+        assert torch.equal(bits(chunk_ssm(one, one, x["v"], x["gt"], x["g"])),
+                           bits(chunk_ssm(one.contiguous(), one.contiguous(), x["v"], x["gt"], x["g"])))
 
 
 def test_mixed_types_take_the_widest():
