@@ -932,25 +932,24 @@ int ssm_tc_bwd(const SsmArgs& s, cudaStream_t st) {
         if (!aligned16(p)) return PALIMPSA_E_ALIGN;
     TcArgs g = tc_args(s, true);
     CUtensorMap q{}, k{}, v{}, d{};
+    const bool wide = padded(a.K) == 128;
+    // ahead of the tensor maps: a call of the runtime makes the device's context current in a thread that has not used it yet
+    // (autograd's, where every allocation came from a cache), and the driver encodes no map without one
+    if (!(wide ? allow_smem<ssm_grad_tc_kernel<128>>(grad_smem<128>()) : allow_smem<ssm_grad_tc_kernel<64>>(grad_smem<64>())))
+        return PALIMPSA_E_LAUNCH;
     if (a.total_tokens > 0 && (!token_map(&q, a.q, a.total_tokens, a.Hq, a.K, a.q_stride) ||
                                !token_map(&k, a.k, a.total_tokens, a.Hq, a.K, a.k_stride) ||
                                !token_map(&v, a.v, a.total_tokens, a.H, a.V, a.v_stride) ||
                                !token_map(&d, a.d_o, a.total_tokens, a.H, a.V, (long long)a.H * a.V)))
         return PALIMPSA_E_LAUNCH;
-    const bool wide = padded(a.K) == 128;
     if (a.num_seqs > 0)
         if (int rc = wide ? launch_walk<128, true>(g, q, d, st) : launch_walk<64, true>(g, q, d, st)) return rc;
     if (s.chunks == 0) return PALIMPSA_OK;
     g.splits = grad_shares(a, s.chunks);
     g.part_qk = reinterpret_cast<float*>(g.grad + image_bytes(a, s.chunks) * 2);
     const dim3 grid(s.chunks, a.Hq, g.splits);
-    if (wide) {
-        if (!allow_smem<ssm_grad_tc_kernel<128>>(grad_smem<128>())) return PALIMPSA_E_LAUNCH;
-        ssm_grad_tc_kernel<128><<<grid, THREADS, grad_smem<128>(), st>>>(g, q, k, v, d);
-    } else {
-        if (!allow_smem<ssm_grad_tc_kernel<64>>(grad_smem<64>())) return PALIMPSA_E_LAUNCH;
-        ssm_grad_tc_kernel<64><<<grid, THREADS, grad_smem<64>(), st>>>(g, q, k, v, d);
-    }
+    if (wide) ssm_grad_tc_kernel<128><<<grid, THREADS, grad_smem<128>(), st>>>(g, q, k, v, d);
+    else ssm_grad_tc_kernel<64><<<grid, THREADS, grad_smem<64>(), st>>>(g, q, k, v, d);
     if (int rc = launched()) return rc;
     if (g.splits > 1) {
         const long long n = a.total_tokens * a.Hq * a.K / 8;

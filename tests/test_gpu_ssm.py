@@ -302,6 +302,29 @@ def test_captured_training_step_repeats_the_eager_one():
             assert torch.equal(a, b)
 
 
+def test_backward_in_a_thread_that_has_not_used_the_device():
+    """Autograd's thread with every allocation cached: the first thing it does with the device is this backward."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from palimpsa_b200.ops import chunk_ssm
+r = lambda *s: torch.randn(*s, device='cuda', dtype=torch.bfloat16)
+keep = [torch.empty(n, device='cuda', dtype=torch.uint8) for n in (1 << 20, 64 << 20, 256 << 20) for _ in range(8)]
+q, v, gt, g, do = r(2, 256, 1, 64), r(2, 256, 4, 64), r(2, 256, 4), torch.ones(4, device='cuda'), r(2, 256, 4, 64)
+chunk_ssm(q, q, v, gt, g, gt_softplus=True)
+del keep
+v.requires_grad_(True)
+torch.autograd.grad(chunk_ssm(q, q, v, gt, g, gt_softplus=True), v, do)
+torch.cuda.synchronize()
+print('done')
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
 def test_two_calls_on_two_streams():
     from palimpsa_b200.ops import chunk_ssm
     d = [make(s, 2, 260, 4, 2, 64, 64, torch.bfloat16) for s in (13, 14)]
