@@ -17,8 +17,10 @@ namespace palimpsa {
 namespace {
 
 constexpr int WARPS = 4;          // of a CTA: neighbouring stretches of the same channels
-constexpr int FWD_STRETCH = 32;   // tokens a warp walks: 3 rows of 35 are read a second time (L2)
+constexpr int FWD_STRETCH = 64;   // tokens a warp walks: 3 rows of 67 are read a second time (L2)
 constexpr int STATE_CHANNELS = 128;
+constexpr int N = 4;              // channels a lane
+constexpr int BATCH = 8;          // rows (of x and dy together) asked for while as many are worked on
 
 struct ConvArgs {
     palimpsa_short_conv a;
@@ -62,9 +64,37 @@ __device__ __forceinline__ void last_inputs(const palimpsa_short_conv& a, int n,
     for (int j = 0; j < W - 1; ++j) st1(a.state_out, ((long long)n * a.D + c) * (W - 1) + j, x[j][0], DT);
 }
 
+// Four channels of a row as they lie in memory: what waits in registers for its turn.
+template <int DT>
+struct Raw {
+    unsigned u[DT == PALIMPSA_F32 ? 4 : 2];
+    __device__ __forceinline__ void ld(const void* base, long long idx) {
+        if constexpr (DT == PALIMPSA_F32) {
+            const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + idx);
+            u[0] = x.x, u[1] = x.y, u[2] = x.z, u[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(base) + idx);
+            u[0] = x.x, u[1] = x.y;
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+        if constexpr (DT == PALIMPSA_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(u[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float2 f;
+                if (DT == PALIMPSA_BF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]));
+                else f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            }
+        }
+    }
+};
+
 template <int DT, int W, bool SILU>
 __global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) {
-    constexpr int N = DT == PALIMPSA_F32 ? 4 : 8;
     const palimpsa_short_conv& a = g.a;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     if ((int)blockIdx.y >= g.token_ctas) {  // final states
@@ -96,33 +126,45 @@ __global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) 
             for (; t < b; ++t) st_n<DT, N>(a.y, t * a.D + c, live, g.vec, zero);
             continue;
         }
-        float win[W][N];  // win[W-1]: the newest
+        float win[W - 1][N];  // the inputs in front of token t, the newest last
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j + 1]);
-        constexpr int BATCH = 8;  // rows asked for before the first is used
-        for (; t < b; t += BATCH) {
-            float x[BATCH][N];
+        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j]);
+        auto token = [&](long long u, const float (&x)[N]) __attribute__((always_inline)) {
+            float y[N];
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i)
-                if (t + i < b) ld_n<DT, N>(a.x, (t + i) * a.x_stride + c, live, g.vec, x[i]);
+            for (int e = 0; e < N; ++e) {
+                float p = fmaf(wt[W - 1][e], x[e], bias[e]);
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                if (t + i >= b) break;
-                float y[N];
+                for (int j = 0; j < W - 1; ++j) p = fmaf(wt[j][e], win[j][e], p);
+                y[e] = SILU ? p * sigmoid_of<DT>(p) : p;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
+                for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
+                win[W - 2][e] = x[e];
+            }
+            st_n<DT, N>(a.y, u * a.D + c, live, g.vec, y);
+        };
+        if (g.vec) {  // rows asked for two batches ahead of their use
+            Raw<DT> next[BATCH];
+            const long long full = t + (b - t) / BATCH * BATCH;
+            if (t < full)
 #pragma unroll
-                    for (int j = 0; j < W - 1; ++j) win[j][e] = win[j + 1][e];
-                    win[W - 1][e] = x[i][e];
-                    float p = bias[e];
+                for (int i = 0; i < BATCH; ++i) next[i].ld(a.x, (t + i) * a.x_stride + c);
+            for (; t < full; t += BATCH) {
+                float x[BATCH][N];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) p = fmaf(wt[j][e], win[j][e], p);
-                    y[e] = SILU ? p * sigmoid_of<DT>(p) : p;
-                }
-                st_n<DT, N>(a.y, (t + i) * a.D + c, live, g.vec, y);
+                for (int i = 0; i < BATCH; ++i) next[i].get(x[i]);
+                if (t + BATCH < full)
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) next[i].ld(a.x, (t + BATCH + i) * a.x_stride + c);
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) token(t + i, x[i]);
             }
         }
-        t = b;
+        for (; t < b; ++t) {
+            float x[N];
+            ld_n<DT, N>(a.x, t * a.x_stride + c, live, g.vec, x);
+            token(t, x);
+        }
     }
 }
 
@@ -131,7 +173,8 @@ template <int DT, int W, bool SILU>
 __device__ __forceinline__ float d_pre(const palimpsa_short_conv& a, int n, long long bos, long long t, long long c) {
     float p = a.bias ? a.bias[c] : 0.f, x[1];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
+    for (int i = 0; i < W; ++i) {
+        const int j = (i + W - 1) % W;  // the newest first, as everywhere here
         ld_input<DT, W, 1>(a, n, bos, t - (W - 1) + j, c, 1, false, x);
         p = fmaf(a.weight[c * W + j], x[0], p);
     }
@@ -143,7 +186,6 @@ __device__ __forceinline__ float d_pre(const palimpsa_short_conv& a, int n, long
 
 template <int DT, int W, bool SILU>
 __global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) {
-    constexpr int N = 4;
     __shared__ float sums[WARPS][W + 1][32 * N];
     const palimpsa_short_conv& a = g.a;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -201,69 +243,85 @@ __global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) 
             for (; t < b; ++t) st_n<DT, N>(a.dx, t * a.D + c, live, g.vec, zero);
             continue;
         }
-        float win[W][N], d[W][N];  // inputs, and d_t of the last W tokens
+        float win[W - 1][N], d[W - 1][N];  // the inputs in front of token t, and the d_t of the tokens in front of it
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j + 1]);
+        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j]);
 #pragma unroll
-        for (int j = 0; j < W; ++j)
+        for (int j = 0; j < W - 1; ++j)
 #pragma unroll
             for (int e = 0; e < N; ++e) d[j][e] = 0.f;
-        const long long a0 = t, last = b + W - 1;  // tokens t .. last-1, those past eos with d = 0
-        constexpr int BATCH = 4;
-        for (; t < last; t += BATCH) {
-            float x[BATCH][N], dy[BATCH][N];
+        const long long a0 = t, last = b + W - 1;  // tokens a0 .. last-1, those past eos with d = 0
+        // one token: its d, its share of the weights' gradients where it is this run's, and dx of the token W-1 before it
+        auto token = [&](auto own, const float (&x)[N], const float (&dy)[N], float (&dx)[N]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                if (t + i < last && t + i < s.eos) {
-                    ld_n<DT, N>(a.x, (t + i) * a.x_stride + c, live, g.vec, x[i]);
-                    ld_n<DT, N>(a.dy, (t + i) * a.D + c, live, g.vec, dy[i]);
-                } else {
+            for (int e = 0; e < N; ++e) {
+                float dp = dy[e];
+                if (SILU) {
+                    float p = fmaf(wt[W - 1][e], x[e], bias[e]);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) x[i][e] = dy[i][e] = 0.f;
+                    for (int j = 0; j < W - 1; ++j) p = fmaf(wt[j][e], win[j][e], p);
+                    const float sg = sigmoid_of<DT>(p);
+                    dp *= sg * fmaf(p, 1.f - sg, 1.f);
                 }
+                if constexpr (decltype(own)::value) {
+                    db[e] += dp;
+                    dw[W - 1][e] = fmaf(dp, x[e], dw[W - 1][e]);
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) dw[j][e] = fmaf(dp, win[j][e], dw[j][e]);
+                }
+                // d[j] is that of the token j behind it, which reads it through weight W-1-j
+                dx[e] = wt[0][e] * dp;
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) dx[e] = fmaf(wt[W - 1 - j][e], d[j][e], dx[e]);
+#pragma unroll
+                for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e], d[j][e] = d[j + 1][e];
+                win[W - 2][e] = x[e], d[W - 2][e] = dp;
             }
+        };
+        auto edge = [&](long long u) {  // a token near the run's ends
+            float x[N], dy[N], dx[N];
+            const long long r = u - (W - 1);
+            if (u < s.eos) {
+                ld_n<DT, N>(a.x, u * a.x_stride + c, live, g.vec, x);
+                ld_n<DT, N>(a.dy, u * a.D + c, live, g.vec, dy);
+            } else {
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const long long u = t + i;
-                if (u >= last) break;
-                const bool inside = u < s.eos, own = u < b;
-                float dx[N];
+                for (int e = 0; e < N; ++e) x[e] = dy[e] = 0.f;
+            }
+            if (u < b) token(std::true_type(), x, dy, dx);
+            else token(std::false_type(), x, dy, dx);
+            if (r < a0) return;
+            if (a.dstate_out && u >= s.eos) {  // r is among the last W-1 inputs
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
+                for (int e = 0; e < N; ++e)
+                    if (e < live) dx[e] += ld1<DT>(a.dstate_out, ((long long)s.n * a.D + c + e) * (W - 1) + (u - s.eos));
+            }
+            st_n<DT, N>(a.dx, r * a.D + c, live, g.vec, dx);
+        };
+        for (; t < last && t < a0 + W - 1; ++t) edge(t);
+        if (g.vec && t < b) {
+            constexpr int B2 = BATCH / 2;
+            Raw<DT> nx[B2], nd[B2];
+            const long long full = t + (b - t) / B2 * B2;
+            auto ask = [&](long long u) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int j = 0; j < W - 1; ++j) win[j][e] = win[j + 1][e], d[j][e] = d[j + 1][e];
-                    win[W - 1][e] = x[i][e];
-                    float dp = dy[i][e];
-                    if (SILU) {
-                        float p = bias[e];
+                for (int i = 0; i < B2; ++i) nx[i].ld(a.x, (u + i) * a.x_stride + c), nd[i].ld(a.dy, (u + i) * a.D + c);
+            };
+            if (t < full) ask(t);
+            for (; t < full; t += B2) {
+                float x[B2][N], dy[B2][N];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) p = fmaf(wt[j][e], win[j][e], p);
-                        const float sg = sigmoid_of<DT>(p);
-                        dp *= sg * (1.f + p * (1.f - sg));
-                    }
-                    d[W - 1][e] = inside ? dp : 0.f;
-                    if (own) {
-                        db[e] += dp;
+                for (int i = 0; i < B2; ++i) nx[i].get(x[i]), nd[i].get(dy[i]);
+                if (t + B2 < full) ask(t + B2);
 #pragma unroll
-                        for (int j = 0; j < W; ++j) dw[j][e] = fmaf(dp, win[j][e], dw[j][e]);
-                    }
-                    // token u - (W-1): d[j] is that of token u - (W-1) + j, which reads it through weight W-1-j
-                    dx[e] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < W; ++j) dx[e] = fmaf(wt[W - 1 - j][e], d[j][e], dx[e]);
-                }
-                const long long r = u - (W - 1);
-                if (r >= a0) {
-                    if (a.dstate_out && r >= s.eos - (W - 1)) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e)
-                            if (e < live)
-                                dx[e] += ld1<DT>(a.dstate_out, ((long long)s.n * a.D + c + e) * (W - 1) + (r - (s.eos - (W - 1))));
-                    }
-                    st_n<DT, N>(a.dx, r * a.D + c, live, g.vec, dx);
+                for (int i = 0; i < B2; ++i) {
+                    float dx[N];
+                    token(std::true_type(), x[i], dy[i], dx);
+                    st_n<DT, N>(a.dx, (t + i - (W - 1)) * a.D + c, live, true, dx);
                 }
             }
         }
+        for (; t < last; ++t) edge(t);
         t = b;
     }
 #pragma unroll
@@ -316,9 +374,9 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const palimpsa_short_con
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) x[j] = ld1<DT>(a.state, i * (W - 1) + j);
     x[W - 1] = ld1<DT>(a.x, n * a.x_stride + c);
-    float p = a.bias ? a.bias[c] : 0.f;
+    float p = fmaf(a.weight[c * W + W - 1], x[W - 1], a.bias ? a.bias[c] : 0.f);  // in the order of the prompt's kernel: the same bits
 #pragma unroll
-    for (int j = 0; j < W; ++j) p = fmaf(a.weight[c * W + j], x[j], p);
+    for (int j = 0; j < W - 1; ++j) p = fmaf(a.weight[c * W + j], x[j], p);
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) st1(a.state_out, i * (W - 1) + j, x[j + 1], DT);
     st1(a.y, i, SILU ? p * sigmoid_of<DT>(p) : p, DT);
@@ -378,9 +436,8 @@ int palimpsa_short_conv_fwd(const palimpsa_short_conv* a, void* stream) {
     if (int rc = check(a)) return rc;
     if (a->total_tokens > 0 && !a->y) return PALIMPSA_E_NULL;
     ConvArgs g{*a, FWD_STRETCH, 0, false};
-    const int n = a->io_dtype == PALIMPSA_F32 ? 4 : 8;
-    g.vec = rows_vec(a->x, a->x_stride, n, a->io_dtype) && rows_vec(a->y, a->D, n, a->io_dtype);
-    const long long chunks = (a->D + 32 * n - 1) / (32 * n);
+    g.vec = a->D % N == 0 && rows_vec(a->x, a->x_stride, N, a->io_dtype) && rows_vec(a->y, a->D, N, a->io_dtype);
+    const long long chunks = (a->D + 32 * N - 1) / (32 * N);
     // short batches: shorter stretches, so that more warps share the latency
     while (g.stretch > 8 && a->total_tokens * chunks < (long long)g.stretch * B200_SMS * 16) g.stretch /= 2;
     const long long per = (long long)g.stretch * WARPS, ctas = (a->total_tokens + per - 1) / per;
@@ -403,7 +460,8 @@ int palimpsa_short_conv_bwd(const palimpsa_short_conv* a, void* stream) {
         a->workspace_bytes < palimpsa_short_conv_workspace_bytes(a))
         return PALIMPSA_E_WORKSPACE;
     ConvArgs g{*a, bwd_stretch(*a), 0, false};
-    g.vec = rows_vec(a->x, a->x_stride, 4, a->io_dtype) && rows_vec(a->dx, a->D, 4, a->io_dtype) && rows_vec(a->dy, a->D, 4, a->io_dtype);
+    g.vec = a->D % N == 0 && rows_vec(a->x, a->x_stride, N, a->io_dtype) && rows_vec(a->dx, a->D, N, a->io_dtype) &&
+            rows_vec(a->dy, a->D, N, a->io_dtype);
     const long long parts = bwd_parts(*a), chunks = (a->D + 127) / 128;
     const long long states = a->dstate ? state_ctas(a->num_seqs) : 0;
     g.token_ctas = (int)parts;

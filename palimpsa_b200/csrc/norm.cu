@@ -126,7 +126,12 @@ __global__ void __launch_bounds__(256) norm_finish_kernel(const float* part, int
 
 int launched() { return cudaGetLastError() == cudaSuccess ? PALIMPSA_OK : PALIMPSA_E_LAUNCH; }
 
-constexpr int BWD_CTAS = 4;  // of an SM: each is a row of the workspace
+constexpr int BWD_THREADS = 1024;  // of an SM; each CTA's sums are a row of the workspace
+
+int bwd_ctas(long long D) {
+    const int t = norm_row_threads(D);
+    return BWD_THREADS / (t < 128 ? 128 : t);
+}
 
 }  // namespace
 
@@ -134,7 +139,7 @@ extern "C" {
 
 size_t palimpsa_rms_norm_workspace_bytes(const palimpsa_rms_norm* a) {
     if (!a || a->D <= 0 || a->rows < 0 || a->D > 16384) return 0;
-    return (size_t)(norm_ctas(*a, BWD_CTAS) * a->D) * 4 + 256;
+    return (size_t)(norm_ctas(*a, bwd_ctas(a->D)) * a->D) * 4 + 256;
 }
 
 int palimpsa_rms_norm_fwd(const palimpsa_rms_norm* a, void* stream) {
@@ -167,7 +172,7 @@ int palimpsa_rms_norm_bwd(const palimpsa_rms_norm* a, void* stream) {
         a->workspace_bytes < palimpsa_rms_norm_workspace_bytes(a))
         return PALIMPSA_E_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long long parts = norm_ctas(*a, BWD_CTAS);
+    const long long parts = norm_ctas(*a, bwd_ctas(a->D));
     const int zt = a->res_dtype == NO_RES ? a->io_dtype : a->res_dtype;
     bool vec = a->D % 8 == 0 && rows_vec(a->dy, a->D, 8, a->io_dtype) && rows_vec(a->dx, a->D, 8, a->io_dtype);
     vec = vec && (a->res_dtype == NO_RES ? rows_vec(a->x, a->x_stride, 8, zt) : rows_vec(a->z, a->D, 8, zt));

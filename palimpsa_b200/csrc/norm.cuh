@@ -1,6 +1,6 @@
 // Residual addition and RMS norm: what norm.cu (output in the io type, backward) and norm_quant.cu (8-bit output) share.
 //
-// A row is held by TPR threads (a warp up to 1024 channels, else a CTA), each with NC chunks of 8 neighbouring channels in
+// A row is held by TPR threads (a warp up to 512 channels, else a CTA), each with NC chunks of 8 neighbouring channels in
 // registers, so that it is read once whatever is done with it.  A CTA takes row after row and keeps its channels' weights.
 #pragma once
 
@@ -100,10 +100,10 @@ int norm_dispatch(const palimpsa_rms_norm& a, F&& f) {
         using std::integral_constant;
         if (a.D <= 256) return f(dt, rt, integral_constant<int, 32>(), integral_constant<int, 1>());
         if (a.D <= 512) return f(dt, rt, integral_constant<int, 32>(), integral_constant<int, 2>());
-        if (a.D <= 1024) return f(dt, rt, integral_constant<int, 32>(), integral_constant<int, 4>());
-        if (a.D <= 2048) return f(dt, rt, integral_constant<int, 128>(), integral_constant<int, 2>());
+        if (a.D <= 1024) return f(dt, rt, integral_constant<int, 128>(), integral_constant<int, 1>());
+        if (a.D <= 2048) return f(dt, rt, integral_constant<int, 256>(), integral_constant<int, 1>());
         if (a.D <= 4096) return f(dt, rt, integral_constant<int, 256>(), integral_constant<int, 2>());
-        if (a.D <= 8192) return f(dt, rt, integral_constant<int, 256>(), integral_constant<int, 4>());
+        if (a.D <= 8192) return f(dt, rt, integral_constant<int, 512>(), integral_constant<int, 2>());
         return f(dt, rt, integral_constant<int, 512>(), integral_constant<int, 4>());
     };
     using F32 = std::integral_constant<int, PALIMPSA_F32>;
@@ -117,7 +117,7 @@ int norm_dispatch(const palimpsa_rms_norm& a, F&& f) {
            : a.io_dtype == PALIMPSA_BF16 ? res(std::integral_constant<int, PALIMPSA_BF16>())
                                          : res(std::integral_constant<int, PALIMPSA_F16>());
 }
-inline int norm_row_threads(long long D) { return D <= 1024 ? 32 : D <= 2048 ? 128 : D <= 8192 ? 256 : 512; }
+inline int norm_row_threads(long long D) { return D <= 512 ? 32 : D <= 1024 ? 128 : D <= 4096 ? 256 : 512; }
 inline int norm_check(const palimpsa_rms_norm* a) {
     if (!a) return PALIMPSA_E_NULL;
     if (a->struct_size != sizeof(palimpsa_rms_norm)) return PALIMPSA_E_VERSION;

@@ -31,14 +31,31 @@ __device__ __forceinline__ bool in_doubt(float t) {
     return fabsf(m - floorf(m) - 0.5f) < 0x1p-14f;  // |t| <= 127: an error of 2^-15.4
 }
 template <int OUT>
-__device__ __forceinline__ unsigned eight_bits(float t, double exact_num, double factor) {
-    if (OUT == PALIMPSA_NORM_E4M3) {
-        if (in_doubt<OUT>(t)) t = to_odd(exact_num * factor);
-        return (unsigned)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
-    }
-    int q = in_doubt<OUT>(t) ? __double2int_rn(exact_num * factor) : __float2int_rn(t);
-    q = q > 127 ? 127 : q < -127 ? -127 : q;
-    return (unsigned)q & 0xffu;
+__device__ __forceinline__ unsigned eight_bits(float t) {
+    if (OUT == PALIMPSA_NORM_E4M3) return (unsigned)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+    const int q = __float2int_rn(t);
+    return (unsigned)(q > 127 ? 127 : q < -127 ? -127 : q) & 0xffu;
+}
+template <int OUT>
+__device__ __forceinline__ unsigned pair_bits(float t, float u) {
+    if (OUT == PALIMPSA_NORM_E4M3) return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(t, u), __NV_SATFINITE, __NV_E4M3);
+    return eight_bits<OUT>(t) | eight_bits<OUT>(u) << 8;
+}
+
+// 1 / sqrt(x) and 1 / s in 64 bits, to a few of their last bits: two steps of Newton's method from the float32 value (2^-22, then
+// 2^-43, then 2^-53), where that is in range.  The library's square root and division take ten times as many instructions, for
+// 8 to 32 elements a thread.
+__device__ __forceinline__ double rsqrt64(double x) {
+    if (!(x > 1e-30 && x < 1e30)) return 1. / sqrt(x);
+    double r = rsqrtf((float)x);
+    r = r * fma(-0.5 * x * r, r, 1.5);
+    return r * fma(-0.5 * x * r, r, 1.5);
+}
+__device__ __forceinline__ double rcp64(float s) {
+    if (!(s > 1e-35f && s < 1e30f)) return 1. / (double)s;
+    double r = __frcp_rn(s);
+    r = fma(r, fma(-(double)s, r, 1.), r);
+    return fma(r, fma(-(double)s, r, 1.), r);
 }
 
 struct Top {  // a value and its remainder, m + l exactly; the largest by m, then by l
@@ -57,6 +74,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_quant_kernel(const N
     const palimpsa_rms_norm& a = g.a;
     const Chunks<NC> ch(threadIdx.x % TPR, TPR, a.D);
     const int blocks = a.block ? (int)((a.D + a.block - 1) / a.block) : 1;
+    const double per_channel = 1. / (double)a.D;
     float w[NC][8];
     ld_weight<NC>(a.weight, ch, w);
     for (long long row = (long long)blockIdx.x * RPC + threadIdx.x / TPR; row < a.rows; row += (long long)gridDim.x * RPC) {
@@ -76,7 +94,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_quant_kernel(const N
             }
         }
         row_add<TPR>(ss, scratch);
-        const double r = 1. / sqrt(ss[0] / (double)a.D + a.eps);
+        const double r = rsqrt64(fma(ss[0], per_channel, a.eps));
         // the group that shares a scale: block/8 neighbouring lanes, or the row
         const int lanes = a.block ? a.block / 8 : 32;
         if (!a.block) {
@@ -103,8 +121,8 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_quant_kernel(const N
         for (int i = 0; i < NC; ++i) {
             if (i == 0 || a.block) {
                 const double largest = ((double)top[i].m + (double)top[i].l) * r;
-                const float s = (float)((largest < 0x1p-100 ? 0x1p-100 : largest) / TOP);
-                factor = r / (double)s;
+                const float s = (float)((largest < 0x1p-100 ? 0x1p-100 : largest) * (1. / TOP));
+                factor = r * rcp64(s);
                 factor32 = (float)factor;
                 if (a.block) {
                     if (ch.live[i] > 0 && (threadIdx.x & (lanes - 1)) == 0) a.scale[row * blocks + ch.c[i] / a.block] = s;
@@ -112,12 +130,29 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_quant_kernel(const N
                     a.scale[row] = s;
                 }
             }
-            unsigned q[2] = {0, 0};
+            float t[8];
+            bool doubt = false;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float hi = z[i][e] * w[i][e];
-                q[e / 4] |= eight_bits<OUT>(hi * factor32, (double)z[i][e] * (double)w[i][e], factor) << (8 * (e % 4));
+                t[e] = z[i][e] * w[i][e] * factor32;
+                doubt |= in_doubt<OUT>(t[e]);
             }
+            if (doubt) {
+#pragma unroll 1
+                for (int e = 0; e < 8; ++e) {
+                    float x = 0.f, y = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k == e) x = z[i][k], y = w[i][k];
+                    const float odd = to_odd((double)x * (double)y * factor);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k == e) t[k] = odd;
+                }
+            }
+            unsigned q[2];
+            q[0] = pair_bits<OUT>(t[0], t[1]) | pair_bits<OUT>(t[2], t[3]) << 16;
+            q[1] = pair_bits<OUT>(t[4], t[5]) | pair_bits<OUT>(t[6], t[7]) << 16;
             if (ch.live[i] > 0) {
                 unsigned char* y = static_cast<unsigned char*>(a.y) + row * a.D + ch.c[i];
                 if (g.vec) {
