@@ -20,7 +20,7 @@ constexpr int WARPS = 4;          // of a CTA: neighbouring stretches of the sam
 constexpr int FWD_STRETCH = 64;   // tokens a warp walks: 3 rows of 67 are read a second time (L2)
 constexpr int STATE_CHANNELS = 128;
 constexpr int N = 4;              // channels a lane
-constexpr int BATCH = 8;          // rows (of x and dy together) asked for while as many are worked on
+constexpr int BATCH = 8;          // rows (of x and dy together) worked on while as many or more are on their way
 
 struct ConvArgs {
     palimpsa_short_conv a;
@@ -36,19 +36,51 @@ __device__ __forceinline__ float sigmoid_of(float x) {
     return rcp_approx(1.f + __expf(-x));
 }
 
-// Input `t` of the sequence (bos..): a row of x, or what the state holds in front of it.
-template <int DT, int W, int N>
-__device__ __forceinline__ void ld_input(const palimpsa_short_conv& a, int n, long long bos, long long t, long long c, int live,
-                                         bool vec, float (&x)[N]) {
-    if (t >= bos) {
-        ld_n<DT, N>(a.x, t * a.x_stride + c, live, vec, x);
-    } else if (a.state) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            x[i] = i < live ? ld1<DT>(a.state, ((long long)n * a.D + c + i) * (W - 1) + (W - 1 + (t - bos))) : 0.f;
+// The channels of a lane: four neighbours where rows may be read that way (VEC), else 32 apart, so that a warp's single
+// accesses are neighbours (with four neighbours each: 30 -> 46 us forward at 777 channels of float32).
+template <bool VEC>
+struct Lane {
+    static constexpr int STEP = VEC ? 1 : 32;
+    long long c;  // first channel
+    int live;     // channels there are
+    __device__ __forceinline__ Lane(long long base, int lane, long long D) {
+        c = base + (VEC ? 4 * lane : lane);
+        const long long left = (D - c + STEP - 1) / STEP;
+        live = left < 0 ? 0 : left > 4 ? 4 : (int)left;
+    }
+};
+template <int DT, bool VEC>
+__device__ __forceinline__ void ld_row(const void* base, long long row, const Lane<VEC>& l, float (&x)[4]) {
+    if constexpr (VEC) {
+        ld_n<DT, 4>(base, row + l.c, 4, true, x);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = 0.f;
+        for (int e = 0; e < 4; ++e) x[e] = e < l.live ? ld1<DT>(base, row + l.c + 32 * e) : 0.f;
+    }
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ void st_row(void* base, long long row, const Lane<VEC>& l, const float (&x)[4]) {
+    if constexpr (VEC) {
+        st_n<DT, 4>(base, row + l.c, 4, true, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < l.live) st1(base, row + l.c + 32 * e, x[e], DT);
+    }
+}
+// Input `t` of the sequence (bos..) in one channel: a row of x, or what the state holds in front of it.
+template <int DT, int W>
+__device__ __forceinline__ float input_at(const palimpsa_short_conv& a, int n, long long bos, long long t, long long c) {
+    if (t >= bos) return ld1<DT>(a.x, t * a.x_stride + c);
+    return a.state ? ld1<DT>(a.state, ((long long)n * a.D + c) * (W - 1) + (W - 1 + (t - bos))) : 0.f;
+}
+template <int DT, int W, bool VEC>
+__device__ __forceinline__ void ld_input(const palimpsa_short_conv& a, int n, long long bos, long long t, const Lane<VEC>& l, float (&x)[4]) {
+    if (t >= bos) {
+        ld_row<DT>(a.x, t * a.x_stride, l, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = e < l.live ? input_at<DT, W>(a, n, bos, t, l.c + e * Lane<VEC>::STEP) : 0.f;
     }
 }
 
@@ -57,44 +89,56 @@ template <int DT, int W>
 __device__ __forceinline__ void last_inputs(const palimpsa_short_conv& a, int n, long long c) {
     long long bos, eos;
     seq_span(a.cu_seqlens, a.seq_len, a.total_tokens, n, bos, eos);
-    float x[W - 1][1];
+    float x[W - 1];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) ld_input<DT, W, 1>(a, n, bos, eos - (W - 1) + j, c, 1, false, x[j]);
+    for (int j = 0; j < W - 1; ++j) x[j] = input_at<DT, W>(a, n, bos, eos - (W - 1) + j, c);
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) st1(a.state_out, ((long long)n * a.D + c) * (W - 1) + j, x[j][0], DT);
+    for (int j = 0; j < W - 1; ++j) st1(a.state_out, ((long long)n * a.D + c) * (W - 1) + j, x[j], DT);
 }
 
-// Four channels of a row as they lie in memory: what waits in registers for its turn.
-template <int DT>
-struct Raw {
-    unsigned u[DT == PALIMPSA_F32 ? 4 : 2];
-    __device__ __forceinline__ void ld(const void* base, long long idx) {
-        if constexpr (DT == PALIMPSA_F32) {
-            const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + idx);
-            u[0] = x.x, u[1] = x.y, u[2] = x.z, u[3] = x.w;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(base) + idx);
-            u[0] = x.x, u[1] = x.y;
+// Rows on their way: a lane's four channels of DEPTH rows in shared memory, copied there asynchronously by the lane itself, so
+// that nobody else has to be waited for and no register holds what has not arrived.  (In registers, one batch ahead, 24 KB an SM
+// were under way: 2.9 TB/s.)  16-bit rows that cannot be read four channels at a time have no copy of 2 bytes: loads when used.
+template <int DT, bool VEC, int DEPTH>
+struct Ring {
+    static constexpr bool COPIED = VEC || DT == PALIMPSA_F32;
+    static constexpr int BYTES = DT == PALIMPSA_F32 ? 16 : 8;
+    static constexpr int SIZE = COPIED ? DEPTH * 32 * WARPS * BYTES : 16;
+    char* at;  // this thread's slots
+    __device__ __forceinline__ explicit Ring(char* base) : at(base + threadIdx.x * BYTES) {}
+    __device__ __forceinline__ char* slot(int i) const { return at + (i % DEPTH) * (32 * WARPS * BYTES); }
+    __device__ __forceinline__ void ask(int i, const void* base, long long row, const Lane<VEC>& l) {
+        if constexpr (COPIED) {
+            const char* p = static_cast<const char*>(base) + (row + l.c) * (DT == PALIMPSA_F32 ? 4 : 2);
+            const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(slot(i)));
+            if constexpr (!VEC) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < l.live) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * e), "l"(p + 128 * e) : "memory");
+            } else if constexpr (BYTES == 16) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+            } else {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(p) : "memory");
+            }
         }
     }
-    __device__ __forceinline__ void get(float (&x)[4]) const {
-        if constexpr (DT == PALIMPSA_F32) {
+    __device__ __forceinline__ void take(int i, const void* base, long long row, const Lane<VEC>& l, float (&x)[4]) const {
+        if constexpr (COPIED) {
+            ld_n<DT, 4>(slot(i), 0, 4, true, x);
+            if constexpr (!VEC) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(u[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float2 f;
-                if (DT == PALIMPSA_BF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]));
-                else f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+                for (int e = 1; e < 4; ++e)
+                    if (e >= l.live) x[e] = 0.f;
             }
+        } else {
+            ld_row<DT>(base, row, l, x);
         }
     }
 };
 
-template <int DT, int W, bool SILU>
-__global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) {
+template <int DT, int W, bool SILU, bool VEC>
+__global__ void __launch_bounds__(32 * WARPS, 6) conv_fwd_kernel(const ConvArgs g) {
+    __shared__ __align__(16) char rows[Ring<DT, VEC, 2 * BATCH>::SIZE];
     const palimpsa_short_conv& a = g.a;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     if ((int)blockIdx.y >= g.token_ctas) {  // final states
@@ -103,14 +147,14 @@ __global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) 
                 last_inputs<DT, W>(a, n, c);
         return;
     }
-    const long long c = ((long long)blockIdx.x * 32 + lane) * N;
-    const int live = (int)min((long long)N, a.D - c);  // <= 0: this lane has no channels, but it helps to look up spans
+    const Lane<VEC> l((long long)blockIdx.x * 32 * N, lane, a.D);
+    const int live = l.live;  // 0: this lane has no channels, but it helps to look up spans
     float wt[W][N], bias[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        bias[i] = a.bias && i < live ? a.bias[c + i] : 0.f;
+        bias[i] = a.bias && i < live ? a.bias[l.c + i * l.STEP] : 0.f;
 #pragma unroll
-        for (int j = 0; j < W; ++j) wt[j][i] = i < live ? a.weight[(c + i) * W + j] : 0.f;
+        for (int j = 0; j < W; ++j) wt[j][i] = i < live ? a.weight[(l.c + i * l.STEP) * W + j] : 0.f;
     }
     long long t = ((long long)blockIdx.y * WARPS + w) * g.stretch;
     const long long end = min(t + g.stretch, (long long)a.total_tokens);
@@ -123,12 +167,12 @@ __global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) 
         }
         if (s.n < 0) {
             float zero[N] = {};
-            for (; t < b; ++t) st_n<DT, N>(a.y, t * a.D + c, live, g.vec, zero);
+            for (; t < b; ++t) st_row<DT>(a.y, t * a.D, l, zero);
             continue;
         }
         float win[W - 1][N];  // the inputs in front of token t, the newest last
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j]);
+        for (int j = 0; j < W - 1; ++j) ld_input<DT, W>(a, s.n, s.bos, t - (W - 1) + j, l, win[j]);
         auto token = [&](long long u, const float (&x)[N]) __attribute__((always_inline)) {
             float y[N];
 #pragma unroll
@@ -141,42 +185,48 @@ __global__ void __launch_bounds__(32 * WARPS) conv_fwd_kernel(const ConvArgs g) 
                 for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
                 win[W - 2][e] = x[e];
             }
-            st_n<DT, N>(a.y, u * a.D + c, live, g.vec, y);
+            st_row<DT>(a.y, u * a.D, l, y);
         };
-        if (g.vec) {  // rows asked for two batches ahead of their use
-            Raw<DT> next[BATCH];
-            const long long full = t + (b - t) / BATCH * BATCH;
-            if (t < full)
+        Ring<DT, VEC, 2 * BATCH> ring(rows);
+        const int n = (int)(b - t);
+        auto ask = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < BATCH; ++i) next[i].ld(a.x, (t + i) * a.x_stride + c);
-            for (; t < full; t += BATCH) {
-                float x[BATCH][N];
-#pragma unroll
-                for (int i = 0; i < BATCH; ++i) next[i].get(x[i]);
-                if (t + BATCH < full)
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) next[i].ld(a.x, (t + BATCH + i) * a.x_stride + c);
-#pragma unroll
-                for (int i = 0; i < BATCH; ++i) token(t + i, x[i]);
-            }
-        }
-        for (; t < b; ++t) {
+            for (int i = i0; i < i0 + BATCH; ++i)
+                if (i < n) ring.ask(i, a.x, (t + i) * a.x_stride, l);
+            cp_async_commit();
+        };
+        ask(0);
+        ask(BATCH);
+        for (int i0 = 0; i0 < n; i0 += BATCH) {
+            cp_async_wait<1>();
             float x[N];
-            ld_n<DT, N>(a.x, t * a.x_stride + c, live, g.vec, x);
-            token(t, x);
+            if (i0 + BATCH <= n) {
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    ring.take(i0 + i, a.x, (t + i0 + i) * a.x_stride, l, x);
+                    token(t + i0 + i, x);
+                }
+            } else {
+                for (int i = i0; i < n; ++i) {
+                    ring.take(i, a.x, (t + i) * a.x_stride, l, x);
+                    token(t + i, x);
+                }
+            }
+            ask(i0 + 2 * BATCH);
         }
+        cp_async_wait<0>();
+        t = b;
     }
 }
 
 // d_t of one channel at token t of (n, bos, eos).
 template <int DT, int W, bool SILU>
 __device__ __forceinline__ float d_pre(const palimpsa_short_conv& a, int n, long long bos, long long t, long long c) {
-    float p = a.bias ? a.bias[c] : 0.f, x[1];
+    float p = a.bias ? a.bias[c] : 0.f;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
         const int j = (i + W - 1) % W;  // the newest first, as everywhere here
-        ld_input<DT, W, 1>(a, n, bos, t - (W - 1) + j, c, 1, false, x);
-        p = fmaf(a.weight[c * W + j], x[0], p);
+        p = fmaf(a.weight[c * W + j], input_at<DT, W>(a, n, bos, t - (W - 1) + j, c), p);
     }
     const float dy = ld1<DT>(a.dy, t * a.D + c);
     if (!SILU) return dy;
@@ -184,8 +234,9 @@ __device__ __forceinline__ float d_pre(const palimpsa_short_conv& a, int n, long
     return dy * sg * (1.f + p * (1.f - sg));
 }
 
-template <int DT, int W, bool SILU>
-__global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) {
+template <int DT, int W, bool SILU, bool VEC>
+__global__ void __launch_bounds__(32 * WARPS, 4) conv_bwd_kernel(const ConvArgs g) {
+    __shared__ __align__(16) char rows[2][Ring<DT, VEC, BATCH>::SIZE];
     __shared__ float sums[WARPS][W + 1][32 * N];
     const palimpsa_short_conv& a = g.a;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -216,16 +267,16 @@ __global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) 
         }
         return;
     }
-    const long long c = ((long long)blockIdx.x * 32 + lane) * N;
-    const int live = (int)min((long long)N, a.D - c);
+    const Lane<VEC> l((long long)blockIdx.x * 32 * N, lane, a.D);
+    const int live = l.live;
     float wt[W][N], bias[N], dw[W][N], db[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        bias[i] = a.bias && i < live ? a.bias[c + i] : 0.f;
+        bias[i] = a.bias && i < live ? a.bias[l.c + i * l.STEP] : 0.f;
         db[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-            wt[j][i] = i < live ? a.weight[(c + i) * W + j] : 0.f;
+            wt[j][i] = i < live ? a.weight[(l.c + i * l.STEP) * W + j] : 0.f;
             dw[j][i] = 0.f;
         }
     }
@@ -240,12 +291,12 @@ __global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) 
         }
         if (s.n < 0) {
             float zero[N] = {};
-            for (; t < b; ++t) st_n<DT, N>(a.dx, t * a.D + c, live, g.vec, zero);
+            for (; t < b; ++t) st_row<DT>(a.dx, t * a.D, l, zero);
             continue;
         }
         float win[W - 1][N], d[W - 1][N];  // the inputs in front of token t, and the d_t of the tokens in front of it
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) ld_input<DT, W, N>(a, s.n, s.bos, t - (W - 1) + j, c, live, g.vec, win[j]);
+        for (int j = 0; j < W - 1; ++j) ld_input<DT, W>(a, s.n, s.bos, t - (W - 1) + j, l, win[j]);
 #pragma unroll
         for (int j = 0; j < W - 1; ++j)
 #pragma unroll
@@ -278,57 +329,63 @@ __global__ void __launch_bounds__(32 * WARPS) conv_bwd_kernel(const ConvArgs g) 
                 win[W - 2][e] = x[e], d[W - 2][e] = dp;
             }
         };
-        auto edge = [&](long long u) {  // a token near the run's ends
+        auto edge = [&](long long u) {  // a token behind the run
             float x[N], dy[N], dx[N];
             const long long r = u - (W - 1);
-            if (u < s.eos) {
-                ld_n<DT, N>(a.x, u * a.x_stride + c, live, g.vec, x);
-                ld_n<DT, N>(a.dy, u * a.D + c, live, g.vec, dy);
+            if (u < s.eos) {  // the next run's token: its d is needed here too
+                ld_row<DT>(a.x, u * a.x_stride, l, x);
+                ld_row<DT>(a.dy, u * a.D, l, dy);
             } else {
 #pragma unroll
                 for (int e = 0; e < N; ++e) x[e] = dy[e] = 0.f;
             }
-            if (u < b) token(std::true_type(), x, dy, dx);
-            else token(std::false_type(), x, dy, dx);
+            token(std::false_type(), x, dy, dx);
             if (r < a0) return;
             if (a.dstate_out && u >= s.eos) {  // r is among the last W-1 inputs
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (e < live) dx[e] += ld1<DT>(a.dstate_out, ((long long)s.n * a.D + c + e) * (W - 1) + (u - s.eos));
+                    if (e < live) dx[e] += ld1<DT>(a.dstate_out, ((long long)s.n * a.D + l.c + e * l.STEP) * (W - 1) + (u - s.eos));
             }
-            st_n<DT, N>(a.dx, r * a.D + c, live, g.vec, dx);
+            st_row<DT>(a.dx, r * a.D, l, dx);
         };
-        for (; t < last && t < a0 + W - 1; ++t) edge(t);
-        if (g.vec && t < b) {
-            constexpr int B2 = BATCH / 2;
-            Raw<DT> nx[B2], nd[B2];
-            const long long full = t + (b - t) / B2 * B2;
-            auto ask = [&](long long u) __attribute__((always_inline)) {
+        Ring<DT, VEC, BATCH> rx(rows[0]), rd(rows[1]);
+        constexpr int B2 = BATCH / 2;
+        const int n = (int)(b - a0);
+        auto ask = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < B2; ++i) nx[i].ld(a.x, (u + i) * a.x_stride + c), nd[i].ld(a.dy, (u + i) * a.D + c);
-            };
-            if (t < full) ask(t);
-            for (; t < full; t += B2) {
-                float x[B2][N], dy[B2][N];
+            for (int i = i0; i < i0 + B2; ++i)
+                if (i < n) rx.ask(i, a.x, (a0 + i) * a.x_stride, l), rd.ask(i, a.dy, (a0 + i) * a.D, l);
+            cp_async_commit();
+        };
+        auto row = [&](int i, bool out) __attribute__((always_inline)) {
+            float x[N], dy[N], dx[N];
+            rx.take(i, a.x, (a0 + i) * a.x_stride, l, x);
+            rd.take(i, a.dy, (a0 + i) * a.D, l, dy);
+            token(std::true_type(), x, dy, dx);
+            if (out) st_row<DT>(a.dx, (a0 + i - (W - 1)) * a.D, l, dx);
+        };
+        ask(0);
+        ask(B2);
+        for (int i0 = 0; i0 < n; i0 += B2) {
+            cp_async_wait<1>();
+            if (i0 >= W - 1 && i0 + B2 <= n) {
 #pragma unroll
-                for (int i = 0; i < B2; ++i) nx[i].get(x[i]), nd[i].get(dy[i]);
-                if (t + B2 < full) ask(t + B2);
-#pragma unroll
-                for (int i = 0; i < B2; ++i) {
-                    float dx[N];
-                    token(std::true_type(), x[i], dy[i], dx);
-                    st_n<DT, N>(a.dx, (t + i - (W - 1)) * a.D + c, live, true, dx);
-                }
+                for (int i = 0; i < B2; ++i) row(i0 + i, true);
+            } else {
+                for (int i = i0; i < n && i < i0 + B2; ++i) row(i, i >= W - 1);
             }
+            ask(i0 + 2 * B2);
         }
+        cp_async_wait<0>();
+        t = b;
         for (; t < last; ++t) edge(t);
         t = b;
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) sums[w][j][lane * N + e] = dw[j][e];
-        sums[w][W][lane * N + e] = db[e];
+        for (int j = 0; j < W; ++j) sums[w][j][VEC ? lane * N + e : lane + 32 * e] = dw[j][e];
+        sums[w][W][VEC ? lane * N + e : lane + 32 * e] = db[e];
     }
     __syncthreads();
     float* part = reinterpret_cast<float*>(a.workspace) + (long long)blockIdx.y * (W + 1) * a.D;
@@ -448,7 +505,9 @@ int palimpsa_short_conv_fwd(const palimpsa_short_conv* a, void* stream) {
     g.token_ctas = (int)((a->total_tokens + (long long)g.stretch * WARPS - 1) / ((long long)g.stretch * WARPS));
     const dim3 grid((unsigned)chunks, (unsigned)(g.token_ctas + states));
     return by_type(*a, [&](auto dt, auto w, auto silu) {
-        conv_fwd_kernel<dt.value, w.value, silu.value><<<grid, 32 * WARPS, 0, static_cast<cudaStream_t>(stream)>>>(g);
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (g.vec) conv_fwd_kernel<dt.value, w.value, silu.value, true><<<grid, 32 * WARPS, 0, st>>>(g);
+        else conv_fwd_kernel<dt.value, w.value, silu.value, false><<<grid, 32 * WARPS, 0, st>>>(g);
         return launched();
     });
 }
@@ -469,7 +528,8 @@ int palimpsa_short_conv_bwd(const palimpsa_short_conv* a, void* stream) {
     if (parts + states > 0) {
         const dim3 grid((unsigned)chunks, (unsigned)(parts + states));
         const int rc = by_type(*a, [&](auto dt, auto w, auto silu) {
-            conv_bwd_kernel<dt.value, w.value, silu.value><<<grid, 32 * WARPS, 0, st>>>(g);
+            if (g.vec) conv_bwd_kernel<dt.value, w.value, silu.value, true><<<grid, 32 * WARPS, 0, st>>>(g);
+            else conv_bwd_kernel<dt.value, w.value, silu.value, false><<<grid, 32 * WARPS, 0, st>>>(g);
             return launched();
         });
         if (rc) return rc;

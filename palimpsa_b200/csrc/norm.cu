@@ -11,16 +11,22 @@ namespace palimpsa {
 namespace {
 
 template <int DT, int RT, int TPR, int NC>
-__global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const NormArgs g) {
+__global__ void __launch_bounds__(norm_threads<TPR>(), norm_ctas_per_sm<TPR, NC>()) norm_fwd_kernel(const NormArgs g) {
     constexpr int RPC = norm_threads<TPR>() / TPR;
     __shared__ float scratch[TPR / 32][1];
     const palimpsa_rms_norm& a = g.a;
     const Chunks<NC> ch(threadIdx.x % TPR, TPR, a.D);
     float w[NC][8];
     ld_weight<NC>(a.weight, ch, w);
-    for (long long row = (long long)blockIdx.x * RPC + threadIdx.x / TPR; row < a.rows; row += (long long)gridDim.x * RPC) {
+    const long long step = (long long)gridDim.x * RPC;
+    long long row = (long long)blockIdx.x * RPC + threadIdx.x / TPR;
+    RowZ<DT, RT, NC> next;
+    if (row < a.rows) next.ask(a, row, ch, g.vec);
+    for (; row < a.rows; row += step) {
         float z[NC][8], ss[1] = {0.f};
-        ld_z<DT, RT, NC>(a, g.vec, row, ch, z);
+        const RowZ<DT, RT, NC> now = next;
+        if (row + step < a.rows) next.ask(a, row + step, ch, g.vec);
+        now.take(a, row, ch, g.vec, z);
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -37,7 +43,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_fwd_kernel(const Nor
 }
 
 template <int DT, int RT, int TPR, int NC>
-__global__ void __launch_bounds__(norm_threads<TPR>()) norm_bwd_kernel(const NormArgs g) {
+__global__ void __launch_bounds__(norm_threads<TPR>(), norm_ctas_per_sm<TPR, NC>()) norm_bwd_kernel(const NormArgs g) {
     constexpr int RPC = norm_threads<TPR>() / TPR, ST = RT == NO_RES ? DT : RT;
     __shared__ float scratch[TPR / 32][2];
     __shared__ float sums[RPC > 1 ? RPC : 1][RPC > 1 ? TPR * NC * 8 : 1];
@@ -51,18 +57,29 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) norm_bwd_kernel(const Nor
         for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
     const void* zp = RT == NO_RES ? a.x : a.z;
     const long long zs = RT == NO_RES ? a.x_stride : a.D;
-    for (long long row = (long long)blockIdx.x * RPC + threadIdx.x / TPR; row < a.rows; row += (long long)gridDim.x * RPC) {
+    const long long step = (long long)gridDim.x * RPC;
+    long long row = (long long)blockIdx.x * RPC + threadIdx.x / TPR;
+    RowPart<ST, NC> nz, nr;
+    RowPart<DT, NC> nd;
+    auto ask = [&](long long r) __attribute__((always_inline)) {
+        nz.ask(zp, r * zs, ch, g.vec);
+        nd.ask(a.dy, r * a.D, ch, g.vec);
+        if (a.dz) nr.ask(a.dz, r * a.D, ch, g.vec);
+    };
+    if (row < a.rows) ask(row);
+    for (; row < a.rows; row += step) {
         float z[NC][8], dy[NC][8], dz[NC][8], s[2] = {0.f, 0.f};
+        nz.take(zp, row * zs, ch, g.vec, z);
+        nd.take(a.dy, row * a.D, ch, g.vec, dy);
+        if (a.dz) {
+            nr.take(a.dz, row * a.D, ch, g.vec, dz);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
+            for (int i = 0; i < NC; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[i][e] = dy[i][e] = dz[i][e] = 0.f;
-            if (ch.live[i] > 0) {
-                ld_n<ST, 8>(zp, row * zs + ch.c[i], ch.live[i], g.vec, z[i]);
-                ld_n<DT, 8>(a.dy, row * a.D + ch.c[i], ch.live[i], g.vec, dy[i]);
-                if (a.dz) ld_n<ST, 8>(a.dz, row * a.D + ch.c[i], ch.live[i], g.vec, dz[i]);
-            }
+                for (int e = 0; e < 8; ++e) dz[i][e] = 0.f;
         }
+        if (row + step < a.rows) ask(row + step);
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -126,11 +143,15 @@ __global__ void __launch_bounds__(256) norm_finish_kernel(const float* part, int
 
 int launched() { return cudaGetLastError() == cudaSuccess ? PALIMPSA_OK : PALIMPSA_E_LAUNCH; }
 
-constexpr int BWD_THREADS = 1024;  // of an SM; each CTA's sums are a row of the workspace
-
-int bwd_ctas(long long D) {
-    const int t = norm_row_threads(D);
-    return BWD_THREADS / (t < 128 ? 128 : t);
+// CTAs of the backward, by the width of the rows alone: each one's sums are a row of the workspace.
+long long bwd_parts(const palimpsa_rms_norm& a) {
+    if (a.D <= 256) return norm_ctas<32, 1>(a);
+    if (a.D <= 512) return norm_ctas<32, 2>(a);
+    if (a.D <= 1024) return norm_ctas<128, 1>(a);
+    if (a.D <= 2048) return norm_ctas<128, 2>(a);
+    if (a.D <= 4096) return norm_ctas<256, 2>(a);
+    if (a.D <= 8192) return norm_ctas<512, 2>(a);
+    return norm_ctas<512, 4>(a);
 }
 
 }  // namespace
@@ -139,7 +160,7 @@ extern "C" {
 
 size_t palimpsa_rms_norm_workspace_bytes(const palimpsa_rms_norm* a) {
     if (!a || a->D <= 0 || a->rows < 0 || a->D > 16384) return 0;
-    return (size_t)(norm_ctas(*a, bwd_ctas(a->D)) * a->D) * 4 + 256;
+    return (size_t)(bwd_parts(*a) * a->D) * 4 + 256;
 }
 
 int palimpsa_rms_norm_fwd(const palimpsa_rms_norm* a, void* stream) {
@@ -156,7 +177,7 @@ int palimpsa_rms_norm_fwd(const palimpsa_rms_norm* a, void* stream) {
     const NormArgs g{*a, vec};
     return norm_dispatch(*a, [&](auto dt, auto rt, auto tpr, auto nc) {
         constexpr int T = norm_threads<tpr.value>();
-        norm_fwd_kernel<dt.value, rt.value, tpr.value, nc.value><<<(unsigned)norm_ctas(*a, 2048 / T), T, 0, st>>>(g);
+        norm_fwd_kernel<dt.value, rt.value, tpr.value, nc.value><<<(unsigned)norm_ctas<tpr.value, nc.value>(*a), T, 0, st>>>(g);
         return launched();
     });
 }
@@ -172,7 +193,7 @@ int palimpsa_rms_norm_bwd(const palimpsa_rms_norm* a, void* stream) {
         a->workspace_bytes < palimpsa_rms_norm_workspace_bytes(a))
         return PALIMPSA_E_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long long parts = norm_ctas(*a, bwd_ctas(a->D));
+    const long long parts = bwd_parts(*a);
     const int zt = a->res_dtype == NO_RES ? a->io_dtype : a->res_dtype;
     bool vec = a->D % 8 == 0 && rows_vec(a->dy, a->D, 8, a->io_dtype) && rows_vec(a->dx, a->D, 8, a->io_dtype);
     vec = vec && (a->res_dtype == NO_RES ? rows_vec(a->x, a->x_stride, 8, zt) : rows_vec(a->z, a->D, 8, zt));

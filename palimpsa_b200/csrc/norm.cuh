@@ -61,30 +61,80 @@ struct Chunks {
     }
 };
 
-// z of a row: loads of all chunks first, then the sums.
-template <int DT, int RT, int NC>
-__device__ __forceinline__ void ld_z(const palimpsa_rms_norm& a, bool vec, long long row, const Chunks<NC>& ch, float (&z)[NC][8]) {
-    constexpr int ST = RT == NO_RES ? DT : RT;
-    float r[RT == NO_RES ? 1 : NC][8];
+// 8 channels as they lie in memory: what waits in registers while the row before is worked on.
+template <int DT>
+struct Raw8 {
+    uint4 u[DT == PALIMPSA_F32 ? 2 : 1];
+    __device__ __forceinline__ void ld(const void* base, long long idx) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(base) + idx * (DT == PALIMPSA_F32 ? 4 : 2));
+        u[0] = p[0];
+        if constexpr (DT == PALIMPSA_F32) u[1] = p[1];
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        if constexpr (DT == PALIMPSA_F32) {
+            const unsigned r[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        if (ch.live[i] > 0) {
-            ld_n<DT, 8>(a.x, row * a.x_stride + ch.c[i], ch.live[i], vec, z[i]);
-            if constexpr (RT != NO_RES) ld_n<ST, 8>(a.res, row * a.D + ch.c[i], ch.live[i], vec, r[i]);
+            for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i]);
         } else {
+            const unsigned r[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[i][e] = r[RT == NO_RES ? 0 : i][e] = 0.f;
+            for (int i = 0; i < 4; ++i) {
+                float2 f;
+                if (DT == PALIMPSA_BF16) f = make_float2(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u));
+                else f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            }
         }
     }
-    if constexpr (RT != NO_RES) {
+};
+// One tensor's part of a row: asked for ahead where it can be (vec), else when it is taken.
+template <int DT, int NC>
+struct RowPart {
+    Raw8<DT> raw[NC];
+    __device__ __forceinline__ void ask(const void* base, long long at, const Chunks<NC>& ch, bool vec) {
+        if (!vec) return;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (ch.live[i] > 0) raw[i].ld(base, at + ch.c[i]);
+    }
+    __device__ __forceinline__ void take(const void* base, long long at, const Chunks<NC>& ch, bool vec, float (&x)[NC][8]) const {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
+            if (ch.live[i] <= 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[i][e] = rounded<ST>(z[i][e] + r[i][e]);
-            if (ch.live[i] > 0) st_n<ST, 8>(a.z, row * a.D + ch.c[i], ch.live[i], vec, z[i]);
+                for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+            } else if (vec) {
+                raw[i].get(x[i]);
+            } else {
+                ld_n<DT, 8>(base, at + ch.c[i], ch.live[i], false, x[i]);
+            }
         }
     }
-}
+};
+// z of a row: x, or the sum with the residual as it is stored.
+template <int DT, int RT, int NC>
+struct RowZ {
+    static constexpr int ST = RT == NO_RES ? DT : RT;
+    RowPart<DT, NC> x;
+    RowPart<ST, RT == NO_RES ? 1 : NC> r;
+    __device__ __forceinline__ void ask(const palimpsa_rms_norm& a, long long row, const Chunks<NC>& ch, bool vec) {
+        x.ask(a.x, row * a.x_stride, ch, vec);
+        if constexpr (RT != NO_RES) r.ask(a.res, row * a.D, ch, vec);
+    }
+    __device__ __forceinline__ void take(const palimpsa_rms_norm& a, long long row, const Chunks<NC>& ch, bool vec, float (&z)[NC][8]) const {
+        x.take(a.x, row * a.x_stride, ch, vec, z);
+        if constexpr (RT != NO_RES) {
+            float y[NC][8];
+            r.take(a.res, row * a.D, ch, vec, y);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[i][e] = rounded<ST>(z[i][e] + y[i][e]);
+                if (ch.live[i] > 0) st_n<ST, 8>(a.z, row * a.D + ch.c[i], ch.live[i], vec, z[i]);
+            }
+        }
+    }
+};
 template <int NC>
 __device__ __forceinline__ void ld_weight(const float* weight, const Chunks<NC>& ch, float (&w)[NC][8]) {
 #pragma unroll
@@ -101,7 +151,7 @@ int norm_dispatch(const palimpsa_rms_norm& a, F&& f) {
         if (a.D <= 256) return f(dt, rt, integral_constant<int, 32>(), integral_constant<int, 1>());
         if (a.D <= 512) return f(dt, rt, integral_constant<int, 32>(), integral_constant<int, 2>());
         if (a.D <= 1024) return f(dt, rt, integral_constant<int, 128>(), integral_constant<int, 1>());
-        if (a.D <= 2048) return f(dt, rt, integral_constant<int, 256>(), integral_constant<int, 1>());
+        if (a.D <= 2048) return f(dt, rt, integral_constant<int, 128>(), integral_constant<int, 2>());
         if (a.D <= 4096) return f(dt, rt, integral_constant<int, 256>(), integral_constant<int, 2>());
         if (a.D <= 8192) return f(dt, rt, integral_constant<int, 512>(), integral_constant<int, 2>());
         return f(dt, rt, integral_constant<int, 512>(), integral_constant<int, 4>());
@@ -117,7 +167,6 @@ int norm_dispatch(const palimpsa_rms_norm& a, F&& f) {
            : a.io_dtype == PALIMPSA_BF16 ? res(std::integral_constant<int, PALIMPSA_BF16>())
                                          : res(std::integral_constant<int, PALIMPSA_F16>());
 }
-inline int norm_row_threads(long long D) { return D <= 512 ? 32 : D <= 1024 ? 128 : D <= 4096 ? 256 : 512; }
 inline int norm_check(const palimpsa_rms_norm* a) {
     if (!a) return PALIMPSA_E_NULL;
     if (a->struct_size != sizeof(palimpsa_rms_norm)) return PALIMPSA_E_VERSION;
@@ -130,10 +179,18 @@ inline int norm_check(const palimpsa_rms_norm* a) {
     if (!a->weight) return PALIMPSA_E_NULL;
     return PALIMPSA_OK;
 }
-// CTAs that walk the rows: as many as are resident at once, each row's threads (128 at least) in one.
-inline long long norm_ctas(const palimpsa_rms_norm& a, int per_sm) {
-    const int tpr = norm_row_threads(a.D), rows_per = tpr < 128 ? 128 / tpr : 1;
-    const long long all = (a.rows + rows_per - 1) / rows_per, most = (long long)B200_SMS * per_sm;
+// Threads of an SM that the kernels are compiled for, and CTAs that walk the rows: as many as are resident at once, so that all
+// begin together and end together (with 1.6 and 1.14 times as many: 60 and 110 us instead of what the kernels' comments say).
+template <int TPR, int NC>
+__host__ __device__ constexpr int norm_resident() { return NC == 1 ? 768 : 512; }
+template <int TPR, int NC>
+__host__ __device__ constexpr int norm_ctas_per_sm() {
+    return norm_resident<TPR, NC>() / norm_threads<TPR>() < 1 ? 1 : norm_resident<TPR, NC>() / norm_threads<TPR>();
+}
+template <int TPR, int NC>
+long long norm_ctas(const palimpsa_rms_norm& a) {
+    constexpr int rows_per = norm_threads<TPR>() / TPR;
+    const long long all = (a.rows + rows_per - 1) / rows_per, most = (long long)B200_SMS * norm_ctas_per_sm<TPR, NC>();
     return all < most ? all : most;
 }
 
