@@ -140,21 +140,26 @@ struct Waits {
 };
 
 // ---- states, and backwards their gradients, in front of (behind) every chunk ------------------------------------------------------
-constexpr int WALK_THREADS = 128;
+// What a step costs is a chain -- operand scaled, product, state taken over and written out --, so the step's tiles and scalars are
+// asked for a step ahead (k in two buffers, v as soon as it has been scaled), two CTAs share an SM, and 8 warps share the rows.
+constexpr int WALK_THREADS = 256;  // thread: row k = tid % 128 of the state, 32 columns of d_v by tid / 128
+struct WalkShared {
+    float w[Q];
+    unsigned long long k_loaded[2], v_loaded, made;
+    unsigned slot;
+};
 template <int KP>
-constexpr int walk_smem() { return 1024 + (KP / 64) * BOX + BOX + 2 * BOX + 1024; }
+constexpr int walk_smem() { return 2 * (KP / 64) * BOX + 3 * BOX + (int)sizeof(WalkShared); }
 
 template <int KP, bool BACKWARD>
-__global__ void __launch_bounds__(WALK_THREADS) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(WALK_THREADS, 2) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap) {
-    extern __shared__ char raw[];
-    char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
-    char* kt = sm;                          // k (backwards q): KP/64 boxes
-    char* ws = kt + (KP / 64) * BOX;        // w v in two parts; then the state's image in two parts (KP = 64: its rows 64.. of the
-    char* vt = ws + 2 * BOX;                // product are of what lies behind kt, and not read)
-    float* wt = reinterpret_cast<float*>(vt + BOX);
-    __shared__ __align__(8) unsigned long long loaded, made;
-    __shared__ unsigned slot;
+    // no static shared memory, so that the dynamic part begins on a 1024-byte boundary (checked): two CTAs just fit an SM
+    extern __shared__ __align__(1024) char sm[];
+    char* kt = sm;                          // k (backwards q): two buffers of KP/64 boxes (KP = 64: the product's rows 64.. are of
+    char* ws = kt + 2 * (KP / 64) * BOX;    // what lies behind the box, and not read)
+    char* vt = ws + 2 * BOX;                // ws: w v in two parts; then the state's image in two parts
+    WalkShared& sh = *reinterpret_cast<WalkShared*>(vt + BOX);
     const SsmArgs& s = g.s;
     const palimpsa_ssm& a = s.a;
     const int tid = threadIdx.x, w = tid >> 5, tile = blockIdx.y, nh = blockIdx.x, n = nh / a.H, h = nh - n * a.H, hq = h / (a.H / a.Hq);
@@ -165,44 +170,63 @@ __global__ void __launch_bounds__(WALK_THREADS) ssm_walk_kernel(const TcArgs g, 
     float* end = BACKWARD ? a.dh0 : a.h_out;
     const int planes = BACKWARD ? 2 : g.planes;
     char* images = BACKWARD ? g.grad : g.state;
-    const int k = tid;                      // this thread's row of the state: column k of d_k, 64 columns of d_v
-    const long long at = ((long long)nh * a.V + tile * VT) * a.K + k;
-    float st[VT];
+    const int k = tid & (Q - 1), c0 = (tid >> 7) * 32, v0 = tile * VT + c0;
+    const long long at = ((long long)nh * a.V + v0) * a.K + k;
+    float st[32];
 #pragma unroll
-    for (int v = 0; v < VT; ++v) st[v] = start && k < a.K && tile * VT + v < a.V ? start[at + (long long)v * a.K] : 0.f;
-    if (count > 0) {
+    for (int v = 0; v < 32; ++v) st[v] = start && k < a.K && v0 + v < a.V ? start[at + (long long)v * a.K] : 0.f;
+    Waits wait;
+    if (tc::smem_u32(sm) & 1023u) wait.bad = true;
+    if (count > 0 && !wait.bad) {
         if (tid == 0) {
-            tc::mbar_init(&loaded);
-            tc::mbar_init(&made);
+            for (unsigned long long* b : {&sh.k_loaded[0], &sh.k_loaded[1], &sh.v_loaded, &sh.made}) tc::mbar_init(b);
             tc::mbar_init_fence();
             tc::tma_prefetch_map(&kmap);
             tc::tma_prefetch_map(&vmap);
         }
-        if (w == 0) tc::tmem_alloc(&slot, 64);
+        if (w == 0) tc::tmem_alloc(&sh.slot, 64);
         tc::fence_before_sync();
         __syncthreads();
         tc::fence_after_sync();
-        const unsigned tm = slot;
-        Waits wait;
-        auto load = [&](int i) {  // one thread
-            const SsmChunk ch = ssm_chunk(s, BACKWARD ? last - 1 - i : first + i);
-            tc::mbar_expect_tx(&loaded, (KP / 64 + 1) * BOX);
+        const unsigned tm = sh.slot;
+        auto chunk = [&](int i) { return BACKWARD ? last - 1 - i : first + i; };
+        auto load_k = [&](int i) {  // one thread
+            const SsmChunk ch = ssm_chunk(s, chunk(i));
+            tc::mbar_expect_tx(&sh.k_loaded[i & 1], (KP / 64) * BOX);
 #pragma unroll
-            for (int x = 0; x < KP / 64; ++x) tma_load_3d(kt + x * BOX, &kmap, 64 * x, hq, (int)ch.tok, &loaded);
-            tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &loaded);
+            for (int x = 0; x < KP / 64; ++x)
+                tma_load_3d(kt + ((i & 1) * (KP / 64) + x) * BOX, &kmap, 64 * x, hq, (int)ch.tok, &sh.k_loaded[i & 1]);
         };
-        if (tid == 0) load(0);
-        for (int i = 0; i < count; ++i) {
-            const int c = BACKWARD ? last - 1 - i : first + i;
-            const SsmChunk ch = ssm_chunk(s, c);
-            const long long sc = ((long long)c * a.H + h) * Q;
-            {
-                const float lh = s.lh[sc + tid], ll = s.ll[sc + tid];
-                wt[tid] = BACKWARD ? expf(lh + ll) : expf((s.lh[sc + Q - 1] - lh) + (s.ll[sc + Q - 1] - ll)) * s.dt[sc + tid];
+        auto load_v = [&](int i) {
+            const SsmChunk ch = ssm_chunk(s, chunk(i));
+            tc::mbar_expect_tx(&sh.v_loaded, BOX);
+            tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &sh.v_loaded);
+        };
+        // the scalars of a step: its weights' exponents (one a thread) and its decay
+        float l0 = 0.f, l1 = 0.f, lq0 = 0.f, lq1 = 0.f, dt = 0.f;
+        auto ask = [&](int i) {
+            const long long sc = ((long long)chunk(i) * a.H + h) * Q;
+            lq0 = s.lh[sc + Q - 1], lq1 = s.ll[sc + Q - 1];
+            if (tid < Q) {
+                l0 = s.lh[sc + tid], l1 = s.ll[sc + tid];
+                if (!BACKWARD) dt = s.dt[sc + tid];
             }
-            const float decay = expf(s.lh[sc + Q - 1] + s.ll[sc + Q - 1]);
+        };
+        if (tid == 0) {
+            load_v(0);
+            load_k(0);
+            if (count > 1) load_k(1);
+        }
+        ask(0);
+        for (int i = 0; i < count; ++i) {
+            const int c = chunk(i);
+            const SsmChunk ch = ssm_chunk(s, c);
+            char* kb = kt + (i & 1) * (KP / 64) * BOX;
+            if (tid < Q) sh.w[tid] = BACKWARD ? expf(l0 + l1) : expf((lq0 - l0) + (lq1 - l1)) * dt;
+            const float decay = expf(lq0 + lq1);
+            if (i + 1 < count) ask(i + 1);
             if (tid == 0 && i > 0) bulk_store_read();  // the image of the step before has left shared memory
-            wait.on(&loaded, i & 1);
+            wait.on(&sh.v_loaded, i & 1);
             __syncthreads();
             // w v in two parts: row = token, 8 columns a time
 #pragma unroll
@@ -211,7 +235,7 @@ __global__ void __launch_bounds__(WALK_THREADS) ssm_walk_kernel(const TcArgs g, 
                 float x[8], hi[8], lo[8];
                 if (r < ch.len) {
                     unpack8(*chunk_at(vt, r, cc), x);
-                    const float f = wt[r];
+                    const float f = sh.w[r];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float y = x[e] * f;
@@ -225,77 +249,87 @@ __global__ void __launch_bounds__(WALK_THREADS) ssm_walk_kernel(const TcArgs g, 
                 *chunk_at(ws, r, cc) = pack8(hi);
                 *chunk_at(ws + BOX, r, cc) = pack8(lo);
             }
+            wait.on(&sh.k_loaded[i & 1], (i >> 1) & 1);
             if (ch.len < Q)
 #pragma unroll
-                for (int x = 0; x < KP / 64; ++x) zero_rows(kt + x * BOX, ch.len, tid, WALK_THREADS);
+                for (int x = 0; x < KP / 64; ++x) zero_rows(kb + x * BOX, ch.len, tid, WALK_THREADS);
             tc::fence_async_smem();
             tc::fence_before_sync();
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after_sync();
-                product<true, true>(tm, kt, ws, Q / 16, VT, false);
-                product<true, true>(tm, kt, ws + BOX, Q / 16, VT, true);
-                tc::commit(&made);
+                product<true, true>(tm, kb, ws, Q / 16, VT, false);
+                product<true, true>(tm, kb, ws + BOX, Q / 16, VT, true);
+                tc::commit(&sh.made);
+                if (i + 1 < count) load_v(i + 1);
             }
-            wait.on(&made, i & 1);
+            wait.on(&sh.made, i & 1);
             tc::fence_after_sync();
-            if (tid == 0 && i + 1 < count) load(i + 1);
-            // the image of the state in front of (behind) this chunk: row k, 64 columns, over the operand that is done with
+            if (tid == 0 && i + 2 < count) load_k(i + 2);
+            // the image of the state in front of (behind) this chunk: row k, 32 columns, over the operand that is done with
             if (k < KP) {
 #pragma unroll
-                for (int cc = 0; cc < 8; ++cc) {
+                for (int cc = 0; cc < 4; ++cc) {
                     float hi[8], lo[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         hi[e] = __bfloat162float(__float2bfloat16_rn(st[8 * cc + e]));
                         lo[e] = st[8 * cc + e] - hi[e];
                     }
-                    *chunk_at(ws, k, cc) = pack8(hi);
-                    if (planes == 2) *chunk_at(ws + KP * 128, k, cc) = pack8(lo);
+                    *chunk_at(ws, k, c0 / 8 + cc) = pack8(hi);
+                    if (planes == 2) *chunk_at(ws + KP * 128, k, c0 / 8 + cc) = pack8(lo);
                 }
             }
             tc::fence_async_smem();
             __syncthreads();
             if (tid == 0) bulk_store(images + (((long long)c * a.H + h) * g.tiles + tile) * planes * (KP * 128), ws, planes * (KP * 128));
+            float r[32];
+            tc::tmem_ld32(tm + ((unsigned)(32 * (w & 3)) << 16) + c0, r);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float r[32];
-                tc::tmem_ld32(tm + ((unsigned)(32 * w) << 16) + 32 * half, r);
-#pragma unroll
-                for (int v = 0; v < 32; ++v) st[32 * half + v] = fmaf(decay, st[32 * half + v], r[v]);
-            }
+            for (int v = 0; v < 32; ++v) st[v] = fmaf(decay, st[v], r[v]);
             tc::fence_before_sync();
-        }
-        if (wait.bad) {
-            atomicCAS(&g_ssm_status, 0, 1);
-#pragma unroll
-            for (int v = 0; v < VT; ++v) st[v] = __int_as_float(0x7fc00000);
         }
         if (tid == 0) bulk_store_done();
         __syncthreads();
         if (w == 0) tc::tmem_free(tm, 64);
     }
+    if (wait.bad) {
+        atomicCAS(&g_ssm_status, 0, 1);
+#pragma unroll
+        for (int v = 0; v < 32; ++v) st[v] = __int_as_float(0x7fc00000);
+    }
     if (end && k < a.K)
 #pragma unroll
-        for (int v = 0; v < VT; ++v)
-            if (tile * VT + v < a.V) end[at + (long long)v * a.K] = st[v];
+        for (int v = 0; v < 32; ++v)
+            if (v0 + v < a.V) end[at + (long long)v * a.K] = st[v];
 }
 
 // ---- what a head's exponents are made of, in shared memory -------------------------------------------------------------------------
-struct Scalars {
+struct __align__(16) Scalars {
     float lh[Q], ll[Q], dt[Q], eL[Q], wq[Q];
     float bl[Q];  // e^{L_m-L_j}, m the last token of j's block of 32: what column j brings to rows of later blocks
 };
-__device__ __forceinline__ void load_scalars(Scalars& x, const SsmArgs& s, int c, int h, int tid) {
-    if (tid < Q) {
-        const long long at = ((long long)c * s.a.H + h) * Q, m = at + (tid | 31);
-        const float lh = s.lh[at + tid], ll = s.ll[at + tid];
-        x.lh[tid] = lh, x.ll[tid] = ll, x.dt[tid] = s.dt[at + tid];
-        x.eL[tid] = expf(lh + ll);
-        x.wq[tid] = expf((s.lh[at + Q - 1] - lh) + (s.ll[at + Q - 1] - ll));
-        x.bl[tid] = expf((s.lh[m] - lh) + (s.ll[m] - ll));
+// One token's, asked for a head ahead.
+struct Token {
+    float lh, ll, dt, lqh, lql;
+    __device__ __forceinline__ void ask(const SsmArgs& s, int c, int h, int t) {
+        const long long at = ((long long)c * s.a.H + h) * Q;
+        lh = s.lh[at + t], ll = s.ll[at + t], dt = s.dt[at + t];
+        lqh = s.lh[at + Q - 1], lql = s.ll[at + Q - 1];
     }
+    // by whole warps of 32 neighbouring tokens
+    __device__ __forceinline__ void put(Scalars& x, int t) const {
+        x.lh[t] = lh, x.ll[t] = ll, x.dt[t] = dt;
+        x.eL[t] = expf(lh + ll);
+        x.wq[t] = expf((lqh - lh) + (lql - ll));
+        x.bl[t] = expf((__shfl_sync(0xffffffffu, lh, 31) - lh) + (__shfl_sync(0xffffffffu, ll, 31) - ll));
+    }
+};
+__device__ __forceinline__ void ld4f(const float* p, float (&x)[4]) {
+    const float4 y = *reinterpret_cast<const float4*>(p);
+    x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
 }
+__device__ __forceinline__ void sync_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // 32 values of row r, columns 32 cb .., into an operand of two boxes.
 __device__ __forceinline__ void st_block(char* tile, int r, int cb, const float (&p)[32]) {
 #pragma unroll
@@ -311,9 +345,11 @@ __device__ __forceinline__ void zero_tile(char* tile, int bytes, int tid, int nt
 }
 
 // ---- outputs --------------------------------------------------------------------------------------------------------------------------
-constexpr int THREADS = 256;  // 8 warps: rows 32 (w % 4) .., column half w / 4
+// Two groups of 4 warps take the heads and tiles in turn, each with its own P, v, state and accumulators: what one waits for (its
+// tiles, its products), the other fills.  (One group of 8 warps with the same buffers: 4.8 us a head; so: see below.)
+constexpr int THREADS = 256;
 template <int KP>
-constexpr int out_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * 2 * BOX + 2 * BOX + 2 * KP * 128 + 2 * (int)sizeof(Scalars); }
+constexpr int out_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * (2 * BOX + BOX + KP * 128) + 2 * (int)sizeof(Scalars); }
 
 template <int KP>
 __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, const __grid_constant__ CUtensorMap qmap,
@@ -321,17 +357,18 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
                                                              const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ char raw[];
     char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
-    char* qt = sm;
-    char* kt = qt + (KP / 64) * BOX;
-    char* P = kt + (KP / 64) * BOX;        // two operands of two boxes
-    char* vt = P + 4 * BOX;                // two tiles of v
-    char* ht = vt + 2 * BOX;               // two states (hi)
-    Scalars* sc = reinterpret_cast<Scalars*>(ht + 2 * KP * 128);
-    __shared__ __align__(8) unsigned long long qk_loaded, loaded[2], s_made, made[2];
+    __shared__ __align__(8) unsigned long long qk_loaded, s_made, v_loaded[2], h_loaded[2], made[2];
     __shared__ unsigned slot;
     const SsmArgs& s = g.s;
     const palimpsa_ssm& a = s.a;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, c = blockIdx.x, hq = blockIdx.y, rep = a.H / a.Hq;
+    const int grp = tid >> 7, t = tid & (Q - 1);  // group, and its thread: row t of the chunk
+    char* qt = sm;
+    char* kt = qt + (KP / 64) * BOX;
+    char* P = kt + (KP / 64) * BOX + grp * 2 * BOX;
+    char* vt = kt + (KP / 64) * BOX + 4 * BOX + grp * BOX;
+    char* ht = kt + (KP / 64) * BOX + 6 * BOX + grp * KP * 128;
+    Scalars& x = reinterpret_cast<Scalars*>(kt + (KP / 64) * BOX + 6 * BOX + 2 * KP * 128)[grp];
     const SsmChunk ch = ssm_chunk(s, c);
     if (ch.len == 0) return;
     // this CTA's share of the heads and tiles that read hq
@@ -340,37 +377,42 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
     if (tid == 0) {
         tc::mbar_init(&qk_loaded);
         tc::mbar_init(&s_made);
-        for (int b = 0; b < 2; ++b) tc::mbar_init(&loaded[b]), tc::mbar_init(&made[b]);
+        for (int b = 0; b < 2; ++b) tc::mbar_init(&v_loaded[b]), tc::mbar_init(&h_loaded[b]), tc::mbar_init(&made[b]);
         tc::mbar_init_fence();
     }
     if (w == 0) tc::tmem_alloc(&slot, 512);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const unsigned tm = slot, tS = tm, tY = tm + 128, tU = tm + 256;  // S 128; two Y and two U of 64 columns
-    auto load = [&](int j) {  // one thread
-        const int b = (j - j0) & 1, h = hq * rep + j / g.tiles, tile = j % g.tiles;
-        tc::mbar_expect_tx(&loaded[b], BOX + KP * 128);
-        tma_load_3d(vt + b * BOX, &vmap, tile * VT, h, (int)ch.tok, &loaded[b]);
-        bulk_load(ht + b * KP * 128, g.state + (((long long)c * a.H + h) * g.tiles + tile) * g.planes * (KP * 128), KP * 128, &loaded[b]);
+    const unsigned tm = slot, tS = tm, tY = tm + 128 + 128 * grp, tU = tY + 64;
+    auto load_h = [&](int j) {  // one thread of the group
+        const int h = hq * rep + j / g.tiles, tile = j % g.tiles;
+        tc::mbar_expect_tx(&h_loaded[grp], KP * 128);
+        bulk_load(ht, g.state + (((long long)c * a.H + h) * g.tiles + tile) * g.planes * (KP * 128), KP * 128, &h_loaded[grp]);
+    };
+    auto load_v = [&](int j) {
+        tc::mbar_expect_tx(&v_loaded[grp], BOX);
+        tma_load_3d(vt, &vmap, (j % g.tiles) * VT, hq * rep + j / g.tiles, (int)ch.tok, &v_loaded[grp]);
     };
     if (tid == 0) {
         tc::mbar_expect_tx(&qk_loaded, 2 * (KP / 64) * BOX);
 #pragma unroll
-        for (int x = 0; x < KP / 64; ++x) {
-            tma_load_3d(qt + x * BOX, &qmap, 64 * x, hq, (int)ch.tok, &qk_loaded);
-            tma_load_3d(kt + x * BOX, &kmap, 64 * x, hq, (int)ch.tok, &qk_loaded);
+        for (int b = 0; b < KP / 64; ++b) {
+            tma_load_3d(qt + b * BOX, &qmap, 64 * b, hq, (int)ch.tok, &qk_loaded);
+            tma_load_3d(kt + b * BOX, &kmap, 64 * b, hq, (int)ch.tok, &qk_loaded);
         }
-        load(j0);
-        if (j0 + 1 < j1) load(j0 + 1);
     }
+    int j = j0 + grp;
+    if (t == 0 && j < j1) load_h(j), load_v(j);
+    Token next;
+    if (j < j1) next.ask(s, c, hq * rep + j / g.tiles, t);
     Waits wait;
-    zero_tile(P, 4 * BOX, tid, THREADS);  // the blocks above the diagonal stay zero
+    zero_tile(P, 2 * BOX, t, Q);  // the blocks above the diagonal stay zero
     wait.on(&qk_loaded, 0);
     __syncthreads();
     if (ch.len < Q) {
 #pragma unroll
-        for (int x = 0; x < KP / 64; ++x) zero_rows(qt + x * BOX, ch.len, tid, THREADS), zero_rows(kt + x * BOX, ch.len, tid, THREADS);
+        for (int b = 0; b < KP / 64; ++b) zero_rows(qt + b * BOX, ch.len, tid, THREADS), zero_rows(kt + b * BOX, ch.len, tid, THREADS);
         tc::fence_async_smem();
         __syncthreads();
     }
@@ -380,86 +422,90 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
     }
     wait.on(&s_made, 0);
     tc::fence_after_sync();
-    const int rw = w & 3, half = w >> 2, r = 32 * rw + lane;
+    const int rw = w & 3, r = t;
     const unsigned lanes = (unsigned)(32 * rw) << 16;
-    auto finish = [&](int j) {  // o of head and tile j
-        const int b = (j - j0) & 1, h = hq * rep + j / g.tiles, v0 = (j % g.tiles) * VT;
-        wait.on(&made[b], ((j - j0) >> 1) & 1);
-        tc::fence_after_sync();
-        const float e = sc[b].eL[r], D = a.D ? a.D[h] : 0.f;
-        char* x = vt + b * BOX;
+    for (int n = 0; j < j1; ++n, j += 2) {
+        const int h = hq * rep + j / g.tiles, v0 = (j % g.tiles) * VT;
+        next.put(x, t);
+        const float lh = next.lh, ll = next.ll, e = x.eL[t];
+        sync_group(1 + grp, Q);
+        if (j + 2 < j1) next.ask(s, c, hq * rep + (j + 2) / g.tiles, t);
+        if (t == 0) {
+            wait.on(&h_loaded[grp], n & 1);
+            tc::fence_after_sync();
+            product<false, true>(tU, qt, ht, KP / 16, VT, false);
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int cb = 0; cb <= rw; ++cb) {
+            float p[32];
+            tc::tmem_ld32(tS + lanes + 32 * cb, p);
+            const float* bl = x.bl + 32 * cb;
+            const float* dt = x.dt + 32 * cb;
+            if (cb < rw) {
+                const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int cc = 4 * half + q;
+                for (int i = 0; i < 32; i += 4) {
+                    float b4[4], d4[4];
+                    ld4f(bl + i, b4), ld4f(dt + i, d4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[i + k] *= ai * (b4[k] * d4[k]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float h4[4], l4[4], d4[4];
+                    ld4f(x.lh + 32 * cb + i, h4), ld4f(x.ll + 32 * cb + i, l4), ld4f(dt + i, d4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        p[i + k] = i + k <= lane ? p[i + k] * ex2(((lh - h4[k]) + (ll - l4[k])) * LOG2E) * d4[k] : 0.f;
+                }
+            }
+            st_block(P, r, cb, p);
+        }
+        wait.on(&v_loaded[grp], n & 1);
+        if (ch.len < Q) zero_rows(vt, ch.len, t, Q);
+        tc::fence_async_smem();
+        tc::fence_before_sync();
+        sync_group(1 + grp, Q);
+        if (t == 0) {
+            tc::fence_after_sync();
+            product<false, true>(tY, P, vt, Q / 16, VT, false);
+            tc::commit(&made[grp]);
+        }
+        __syncwarp();
+        wait.on(&made[grp], n & 1);
+        tc::fence_after_sync();
+        if (t == 0 && j + 2 < j1) load_h(j + 2);
+        __syncwarp();
+        const float D = a.D ? a.D[h] : 0.f;
+#pragma unroll
+        for (int cc = 0; cc < 8; ++cc) {
             float y[8], u[8], v[8];
-            tmem_ld8x2(tY + lanes + 64 * b + 8 * cc, tU + lanes + 64 * b + 8 * cc, y, u);
-            unpack8(*chunk_at(x, r, cc), v);
+            tmem_ld8x2(tY + lanes + 8 * cc, tU + lanes + 8 * cc, y, u);
+            unpack8(*chunk_at(vt, r, cc), v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 y[i] = fmaf(e, u[i], fmaf(D, v[i], y[i]));
                 if (wait.bad) y[i] = __int_as_float(0x7fc00000);
             }
-            *chunk_at(x, r, cc) = pack8(y);
+            *chunk_at(vt, r, cc) = pack8(y);
         }
         tc::fence_before_sync();
-        __syncthreads();
+        __syncwarp();  // a warp writes out its own rows
         char* o = static_cast<char*>(a.o) + ((ch.tok * a.H + h) * a.V + v0) * 2;
 #pragma unroll
-        for (int i = 0; i < Q * 8 / THREADS; ++i) {
-            const int row = (tid >> 3) + i * (THREADS / 8), cc = tid & 7;
-            if (row < ch.len && v0 + 8 * cc < a.V) *reinterpret_cast<uint4*>(o + ((long long)row * a.H * a.V + 8 * cc) * 2) = *chunk_at(x, row, cc);
+        for (int i = 0; i < 8; ++i) {
+            const int row = 32 * rw + 4 * i + (lane >> 3), cc = lane & 7;
+            if (row < ch.len && v0 + 8 * cc < a.V) *reinterpret_cast<uint4*>(o + ((long long)row * a.H * a.V + 8 * cc) * 2) = *chunk_at(vt, row, cc);
         }
         tc::fence_async_smem();
-        __syncthreads();
-        if (tid == 0 && j + 2 < j1) load(j + 2);
-    };
-    for (int j = j0; j < j1; ++j) {
-        const int n = j - j0, b = n & 1, h = hq * rep + j / g.tiles;
-        load_scalars(sc[b], s, c, h, tid);
-        wait.on(&loaded[b], (n >> 1) & 1);
-        __syncthreads();
-        if (ch.len < Q) {
-            zero_rows(vt + b * BOX, ch.len, tid, THREADS);
-            tc::fence_async_smem();
-        }
-        if (tid == 0) {
-            tc::fence_after_sync();
-            product<false, true>(tU + 64 * b, qt, ht + b * KP * 128, KP / 16, VT, false);
-        }
-        const Scalars& x = sc[b];
-        char* p = P + b * 2 * BOX;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int cb = 2 * half + k;
-            if (cb > rw) break;
-            float t[32];
-            tc::tmem_ld32(tS + lanes + 32 * cb, t);
-            const float lh = x.lh[r], ll = x.ll[r];
-            if (cb < rw) {
-                const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) t[i] *= ai * (x.bl[32 * cb + i] * x.dt[32 * cb + i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float d = (lh - x.lh[32 * cb + i]) + (ll - x.ll[32 * cb + i]);
-                    t[i] = i <= lane ? t[i] * ex2(d * LOG2E) * x.dt[32 * cb + i] : 0.f;
-                }
-            }
-            st_block(p, r, cb, t);
-        }
-        tc::fence_async_smem();
-        tc::fence_before_sync();
-        __syncthreads();
-        if (tid == 0) {
-            tc::fence_after_sync();
-            product<false, true>(tY + 64 * b, p, vt + b * BOX, Q / 16, VT, false);
-            tc::commit(&made[b]);
-        }
-        if (n > 0) finish(j - 1);
+        sync_group(1 + grp, Q);
+        if (t == 0 && j + 2 < j1) load_v(j + 2);
+        __syncwarp();
     }
-    finish(j1 - 1);
-    if (wait.bad && tid == 0) atomicCAS(&g_ssm_status, 0, 2);
+    if (wait.bad) atomicCAS(&g_ssm_status, 0, 2);
+    tc::fence_before_sync();
     __syncthreads();
     if (w == 0) tc::tmem_free(tm, 512);
 }
@@ -530,6 +576,8 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
         }
         load(h0, 0);
     }
+    Token next;
+    if (tid < Q) next.ask(s, c, h0, tid);
     Waits wait;
     zero_tile(P, 2 * BOX, tid, THREADS);
     wait.on(&qk_loaded, 0);
@@ -558,7 +606,10 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
     int step = 0;
     for (int h = h0; h < h1; ++h) {
         for (int tile = 0; tile < g.tiles; ++tile, ++step) {
-            if (tile == 0) load_scalars(x, s, c, h, tid);
+            if (tile == 0 && tid < Q) {
+                next.put(x, tid);
+                if (h + 1 < h1) next.ask(s, c, h + 1, tid);
+            }
             wait.on(&loaded, step & 1);
             __syncthreads();
             if (ch.len < Q) {
@@ -604,24 +655,36 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 if (cb < rw) {
                     const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float dec = ai * x.bl[32 * cb + i], dt = x.dt[32 * cb + i], q = t[i] * dec;
-                        p[i] = S[k][i] * dec;
-                        t[i] = q * S[k][i];
-                        dS[k][i] = fmaf(q, dt, dS[k][i]);
-                        early = fmaf(t[i], dt, early);
+                    for (int i0 = 0; i0 < 32; i0 += 4) {
+                        float b4[4], d4[4];
+                        ld4f(x.bl + 32 * cb + i0, b4), ld4f(x.dt + 32 * cb + i0, d4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = i0 + e;
+                            const float dec = ai * b4[e], q = t[i] * dec;
+                            p[i] = S[k][i] * dec;
+                            t[i] = q * S[k][i];
+                            dS[k][i] = fmaf(q, d4[e], dS[k][i]);
+                            early = fmaf(t[i], d4[e], early);
+                        }
                     }
                     st_block(P, r, cb, p);
                 } else {
                     float diag = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float d = (lh - x.lh[32 * cb + i]) + (ll - x.ll[32 * cb + i]);
-                        const float dec = i <= lane ? ex2(d * LOG2E) : 0.f, q = i <= lane ? t[i] * dec : 0.f;
-                        if (i == lane) diag = t[i];
-                        p[i] = i <= lane ? S[k][i] * dec : 0.f;
-                        t[i] = q * S[k][i];
-                        dS[k][i] = fmaf(q, x.dt[32 * cb + i], dS[k][i]);
+                    for (int i0 = 0; i0 < 32; i0 += 4) {
+                        float h4[4], l4[4], d4[4];
+                        ld4f(x.lh + 32 * cb + i0, h4), ld4f(x.ll + 32 * cb + i0, l4), ld4f(x.dt + 32 * cb + i0, d4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = i0 + e;
+                            const float dec = i <= lane ? ex2(((lh - h4[e]) + (ll - l4[e])) * LOG2E) : 0.f;
+                            const float q = i <= lane ? t[i] * dec : 0.f;
+                            if (i == lane) diag = t[i];
+                            p[i] = i <= lane ? S[k][i] * dec : 0.f;
+                            t[i] = q * S[k][i];
+                            dS[k][i] = fmaf(q, d4[e], dS[k][i]);
+                        }
                     }
                     st_block(P, r, cb, p);
                     // row i brings sum_{j<t} M_ij to the borders t <= i
@@ -695,6 +758,14 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 if (row < ch.len && v0 + 8 * cc < a.V)
                     *reinterpret_cast<uint4*>(dv + ((long long)row * a.H * a.V + 8 * cc) * 2) = reinterpret_cast<const uint4*>(from)[cc ^ (row & 7)];
             }
+            wait.on(&outer, step & 1);
+            tc::fence_after_sync();
+            tc::fence_async_smem();
+            __syncthreads();  // the tiles, and P behind dv, may be written again
+            if (tid == 0) {
+                if (tile + 1 < g.tiles) load(h, tile + 1);
+                else if (h + 1 < h1) load(h + 1, 0);
+            }
             if (tile + 1 == g.tiles) {  // the head's scalars: thread t of the first 128 has token t, of block b
                 const int t = tid, b = w;
                 float ta = 0.f, tb = 0.f, late = 0.f, own = 0.f, direct = 0.f, dt = 0.f;
@@ -752,14 +823,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                     s.part[n + at] = sums.pb[0] + sums.pb[1] + sums.pb[2] + sums.pb[3];
                     s.part[2 * n + at] = sums.diag[0] + sums.diag[1] + sums.diag[2] + sums.diag[3];
                 }
-            }
-            wait.on(&outer, step & 1);
-            tc::fence_after_sync();
-            tc::fence_async_smem();
-            __syncthreads();  // P, the scalars and the sums may be written again
-            if (tid == 0) {
-                if (tile + 1 < g.tiles) load(h, tile + 1);
-                else if (h + 1 < h1) load(h + 1, 0);
+                __syncthreads();  // the scalars and the sums may be written again
             }
         }
     }
