@@ -118,17 +118,36 @@ __device__ __forceinline__ void zero_rows(char* box, int len, int tid, int nthr)
 }
 
 constexpr unsigned A_MN = 1u << 15, B_MN = tc::IDESC_B_MN_MAJOR;
-// D (+)= A B over `steps` of 16 of the contraction.  K-major operands lie in boxes of 64 columns of the contraction; MN-major ones
-// have its rows 128 bytes apart, 64-column boxes of the other dimension BOX apart.
-template <bool AMN, bool BMN>
-__device__ __forceinline__ void product(unsigned d, const char* a, const char* b, int steps, int n, bool acc) {
-    const unsigned id = tc::idesc_bf16(n) | (AMN ? A_MN : 0) | (BMN ? B_MN : 0);
-    const unsigned sa = tc::smem_u32(a), sb = tc::smem_u32(b);
-    for (int k = 0; k < steps; ++k) {
-        const unsigned along = (k >> 2) * BOX + (k & 3) * 32, down = k * 2048;
-        tc::mma(d, AMN ? tc::desc_mn_sw128(sa + down, BOX) : tc::desc_sw128(sa + along),
-                BMN ? tc::desc_mn_sw128(sb + down, BOX) : tc::desc_sw128(sb + along), id, acc || k > 0);
+// D (+)= A B over STEPS of 16 of the contraction, N columns.  K-major operands lie in boxes of 64 columns of the contraction;
+// MN-major ones have its rows 128 bytes apart, 64-column boxes of the other dimension `abox` and `bbox` bytes apart.
+// A product into an accumulator waits for the one before it, 110 cycles here whatever N is up to 128 (64 x 128 x 16 alone would be
+// 32): so two parts of an operand are columns of one product where TMEM has room, and independent products are issued in turn.
+template <bool AMN, bool BMN, int STEPS, int N>
+struct Product {
+    unsigned d;
+    unsigned long long da, db;
+    __device__ __forceinline__ Product(unsigned d_, const char* a, const char* b, unsigned abox = BOX, unsigned bbox = BOX) : d(d_) {
+        da = AMN ? tc::desc_mn_sw128(tc::smem_u32(a), abox) : tc::desc_sw128(tc::smem_u32(a));
+        db = BMN ? tc::desc_mn_sw128(tc::smem_u32(b), bbox) : tc::desc_sw128(tc::smem_u32(b));
     }
+    __device__ __forceinline__ void step(int k, bool acc) const {
+        const unsigned id = tc::idesc_bf16(N) | (AMN ? A_MN : 0) | (BMN ? B_MN : 0);
+        const int along = ((k >> 2) * BOX + (k & 3) * 32) >> 4, down = (k * 2048) >> 4;  // in the descriptors' units
+        tc::mma(d, da + (AMN ? down : along), db + (BMN ? down : along), id, acc);
+    }
+};
+template <bool AMN, bool BMN, int STEPS, int N>
+__device__ __forceinline__ void product(unsigned d, const char* a, const char* b, bool acc) {
+    const Product<AMN, BMN, STEPS, N> p(d, a, b);
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) p.step(k, k > 0 || acc);
+}
+// The same of two products at a time.
+template <bool AMN, bool BMN, int STEPS, int N>
+__device__ __forceinline__ void products(unsigned d0, const char* a0, const char* b0, unsigned d1, const char* a1, const char* b1, bool acc) {
+    const Product<AMN, BMN, STEPS, N> p(d0, a0, b0), q(d1, a1, b1);
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) p.step(k, k > 0 || acc), q.step(k, k > 0 || acc);
 }
 
 // A wait that has given up once lets all later ones pass (the outputs are NaN by then).
@@ -140,26 +159,29 @@ struct Waits {
 };
 
 // ---- states, and backwards their gradients, in front of (behind) every chunk ------------------------------------------------------
-// What a step costs is a chain -- operand scaled, product, state taken over and written out --, so the step's tiles and scalars are
-// asked for a step ahead (k in two buffers, v as soon as it has been scaled), two CTAs share an SM, and 8 warps share the rows.
-constexpr int WALK_THREADS = 256;  // thread: row k = tid % 128 of the state, 32 columns of d_v by tid / 128
+// Steps are pipelined: while the product of step i runs, the operand of step i+1 is scaled and the image of the state in front of
+// step i is written out, so that a step costs its CUDA-core work and one barrier.  Everything a step writes has two buffers; k and
+// v are asked for one and two steps ahead.  (One step after the other, two CTAs an SM: 66 us for 192 walks of 16 steps, 69 for 64 of
+// 24; so: see ssm_tc_fwd.)
+constexpr int WALK_THREADS = 512;  // thread: row k = tid % 128 of the state, 16 columns of d_v by tid / 128
 struct WalkShared {
-    float w[Q];
-    unsigned long long k_loaded[2], v_loaded, made;
+    float w[2][Q];
+    unsigned long long k_loaded[2], v_loaded[2], made[2];
     unsigned slot;
 };
 template <int KP>
-constexpr int walk_smem() { return 2 * (KP / 64) * BOX + 3 * BOX + (int)sizeof(WalkShared); }
+constexpr int walk_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * BOX + 4 * BOX + 4 * KP * 128 + (int)sizeof(WalkShared); }
 
 template <int KP, bool BACKWARD>
-__global__ void __launch_bounds__(WALK_THREADS, 2) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(WALK_THREADS, 1) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap) {
-    // no static shared memory, so that the dynamic part begins on a 1024-byte boundary (checked): two CTAs just fit an SM
-    extern __shared__ __align__(1024) char sm[];
+    extern __shared__ char raw[];
+    char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
     char* kt = sm;                          // k (backwards q): two buffers of KP/64 boxes (KP = 64: the product's rows 64.. are of
     char* ws = kt + 2 * (KP / 64) * BOX;    // what lies behind the box, and not read)
-    char* vt = ws + 2 * BOX;                // ws: w v in two parts; then the state's image in two parts
-    WalkShared& sh = *reinterpret_cast<WalkShared*>(vt + BOX);
+    char* vt = ws + 4 * BOX;                // ws: w v in two parts, twice
+    char* img = vt + 2 * BOX;               // the state's image in two parts, twice
+    WalkShared& sh = *reinterpret_cast<WalkShared*>(img + 4 * KP * 128);
     const SsmArgs& s = g.s;
     const palimpsa_ssm& a = s.a;
     const int tid = threadIdx.x, w = tid >> 5, tile = blockIdx.y, nh = blockIdx.x, n = nh / a.H, h = nh - n * a.H, hq = h / (a.H / a.Hq);
@@ -170,25 +192,24 @@ __global__ void __launch_bounds__(WALK_THREADS, 2) ssm_walk_kernel(const TcArgs 
     float* end = BACKWARD ? a.dh0 : a.h_out;
     const int planes = BACKWARD ? 2 : g.planes;
     char* images = BACKWARD ? g.grad : g.state;
-    const int k = tid & (Q - 1), c0 = (tid >> 7) * 32, v0 = tile * VT + c0;
+    const int k = tid & (Q - 1), c0 = (tid >> 7) * 16, v0 = tile * VT + c0;
     const long long at = ((long long)nh * a.V + v0) * a.K + k;
-    float st[32];
+    float st[16];
 #pragma unroll
-    for (int v = 0; v < 32; ++v) st[v] = start && k < a.K && v0 + v < a.V ? start[at + (long long)v * a.K] : 0.f;
-    Waits wait;
-    if (tc::smem_u32(sm) & 1023u) wait.bad = true;
-    if (count > 0 && !wait.bad) {
+    for (int v = 0; v < 16; ++v) st[v] = start && k < a.K && v0 + v < a.V ? start[at + (long long)v * a.K] : 0.f;
+    if (count > 0) {
         if (tid == 0) {
-            for (unsigned long long* b : {&sh.k_loaded[0], &sh.k_loaded[1], &sh.v_loaded, &sh.made}) tc::mbar_init(b);
+            for (int b = 0; b < 2; ++b) tc::mbar_init(&sh.k_loaded[b]), tc::mbar_init(&sh.v_loaded[b]), tc::mbar_init(&sh.made[b]);
             tc::mbar_init_fence();
             tc::tma_prefetch_map(&kmap);
             tc::tma_prefetch_map(&vmap);
         }
-        if (w == 0) tc::tmem_alloc(&sh.slot, 64);
+        if (w == 0) tc::tmem_alloc(&sh.slot, 256);
         tc::fence_before_sync();
         __syncthreads();
         tc::fence_after_sync();
         const unsigned tm = sh.slot;
+        Waits wait;
         auto chunk = [&](int i) { return BACKWARD ? last - 1 - i : first + i; };
         auto load_k = [&](int i) {  // one thread
             const SsmChunk ch = ssm_chunk(s, chunk(i));
@@ -199,12 +220,13 @@ __global__ void __launch_bounds__(WALK_THREADS, 2) ssm_walk_kernel(const TcArgs 
         };
         auto load_v = [&](int i) {
             const SsmChunk ch = ssm_chunk(s, chunk(i));
-            tc::mbar_expect_tx(&sh.v_loaded, BOX);
-            tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &sh.v_loaded);
+            tc::mbar_expect_tx(&sh.v_loaded[i & 1], BOX);
+            tma_load_3d(vt + (i & 1) * BOX, &vmap, tile * VT, h, (int)ch.tok, &sh.v_loaded[i & 1]);
         };
-        // the scalars of a step: its weights' exponents (one a thread) and its decay
+        // a step's scalars: its weights (one a thread) and its decay, asked for a step before they are put down
         float l0 = 0.f, l1 = 0.f, lq0 = 0.f, lq1 = 0.f, dt = 0.f;
         auto ask = [&](int i) {
+            if (i >= count) return;
             const long long sc = ((long long)chunk(i) * a.H + h) * Q;
             lq0 = s.lh[sc + Q - 1], lq1 = s.ll[sc + Q - 1];
             if (tid < Q) {
@@ -212,30 +234,21 @@ __global__ void __launch_bounds__(WALK_THREADS, 2) ssm_walk_kernel(const TcArgs 
                 if (!BACKWARD) dt = s.dt[sc + tid];
             }
         };
-        if (tid == 0) {
-            load_v(0);
-            load_k(0);
-            if (count > 1) load_k(1);
-        }
-        ask(0);
-        for (int i = 0; i < count; ++i) {
-            const int c = chunk(i);
-            const SsmChunk ch = ssm_chunk(s, c);
-            char* kb = kt + (i & 1) * (KP / 64) * BOX;
-            if (tid < Q) sh.w[tid] = BACKWARD ? expf(l0 + l1) : expf((lq0 - l0) + (lq1 - l1)) * dt;
-            const float decay = expf(lq0 + lq1);
-            if (i + 1 < count) ask(i + 1);
-            if (tid == 0 && i > 0) bulk_store_read();  // the image of the step before has left shared memory
-            wait.on(&sh.v_loaded, i & 1);
-            __syncthreads();
-            // w v in two parts: row = token, 8 columns a time
+        auto put = [&](int i) {  // step i's weights down, its decay back
+            if (tid < Q) sh.w[i & 1][tid] = BACKWARD ? expf(l0 + l1) : expf((lq0 - l0) + (lq1 - l1)) * dt;
+            return expf(lq0 + lq1);
+        };
+        auto scale = [&](int i, int len) {  // w v in two parts: row = token, 8 columns a time
+            wait.on(&sh.v_loaded[i & 1], (i >> 1) & 1);
+            char* from = vt + (i & 1) * BOX;
+            char* to = ws + (i & 1) * 2 * BOX;
 #pragma unroll
             for (int j = 0; j < Q * 8 / WALK_THREADS; ++j) {
                 const int r = (tid >> 3) + j * (WALK_THREADS / 8), cc = tid & 7;
                 float x[8], hi[8], lo[8];
-                if (r < ch.len) {
-                    unpack8(*chunk_at(vt, r, cc), x);
-                    const float f = sh.w[r];
+                if (r < len) {
+                    unpack8(*chunk_at(from, r, cc), x);
+                    const float f = sh.w[i & 1][r];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float y = x[e] * f;
@@ -246,61 +259,105 @@ __global__ void __launch_bounds__(WALK_THREADS, 2) ssm_walk_kernel(const TcArgs 
 #pragma unroll
                     for (int e = 0; e < 8; ++e) hi[e] = lo[e] = 0.f;
                 }
-                *chunk_at(ws, r, cc) = pack8(hi);
-                *chunk_at(ws + BOX, r, cc) = pack8(lo);
+                *chunk_at(to, r, cc) = pack8(hi);
+                *chunk_at(to + BOX, r, cc) = pack8(lo);
             }
-            wait.on(&sh.k_loaded[i & 1], (i >> 1) & 1);
-            if (ch.len < Q)
+            if (len < Q) {
+                wait.on(&sh.k_loaded[i & 1], (i >> 1) & 1);
 #pragma unroll
-                for (int x = 0; x < KP / 64; ++x) zero_rows(kb + x * BOX, ch.len, tid, WALK_THREADS);
-            tc::fence_async_smem();
-            tc::fence_before_sync();
-            __syncthreads();
-            if (tid == 0) {
-                tc::fence_after_sync();
-                product<true, true>(tm, kb, ws, Q / 16, VT, false);
-                product<true, true>(tm, kb, ws + BOX, Q / 16, VT, true);
-                tc::commit(&sh.made);
-                if (i + 1 < count) load_v(i + 1);
+                for (int x = 0; x < KP / 64; ++x) zero_rows(kt + ((i & 1) * (KP / 64) + x) * BOX, len, tid, WALK_THREADS);
             }
-            wait.on(&sh.made, i & 1);
+        };
+        auto multiply = [&](int i) {  // one thread
             tc::fence_after_sync();
-            if (tid == 0 && i + 2 < count) load_k(i + 2);
-            // the image of the state in front of (behind) this chunk: row k, 32 columns, over the operand that is done with
+            wait.on(&sh.k_loaded[i & 1], (i >> 1) & 1);
+            const char* kb = kt + (i & 1) * (KP / 64) * BOX;
+            const char* wb = ws + (i & 1) * 2 * BOX;
+            product<true, true, Q / 16, 2 * VT>(tm + 128 * (i & 1), kb, wb, false);  // both parts: 64 columns each
+            tc::commit(&sh.made[i & 1]);
+        };
+        if (tid == 0) {
+            for (int i = 0; i < 2 && i < count; ++i) load_v(i), load_k(i);
+        }
+        ask(0);
+        float decay = put(0), decay1 = 1.f;
+        ask(1);
+        if (count > 1) decay1 = put(1);
+        ask(2);
+        __syncthreads();
+        scale(0, ssm_chunk(s, chunk(0)).len);
+        tc::fence_async_smem();
+        tc::fence_before_sync();
+        __syncthreads();
+        if (tid == 0) {
+            multiply(0);
+            if (count > 2) load_v(2);
+        }
+        for (int i = 0; i < count; ++i) {
+            const bool more = i + 1 < count;
+            if (more) scale(i + 1, ssm_chunk(s, chunk(i + 1)).len);
+            // the image of the state in front of (behind) this chunk: row k, 16 columns
+            char* to = img + (i & 1) * 2 * KP * 128;
             if (k < KP) {
 #pragma unroll
-                for (int cc = 0; cc < 4; ++cc) {
+                for (int cc = 0; cc < 2; ++cc) {
                     float hi[8], lo[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         hi[e] = __bfloat162float(__float2bfloat16_rn(st[8 * cc + e]));
                         lo[e] = st[8 * cc + e] - hi[e];
                     }
-                    *chunk_at(ws, k, c0 / 8 + cc) = pack8(hi);
-                    if (planes == 2) *chunk_at(ws + KP * 128, k, c0 / 8 + cc) = pack8(lo);
+                    *chunk_at(to, k, c0 / 8 + cc) = pack8(hi);
+                    if (planes == 2) *chunk_at(to + KP * 128, k, c0 / 8 + cc) = pack8(lo);
+                }
+            }
+            float decay2 = 1.f;
+            if (i + 2 < count) {
+                decay2 = put(i + 2);  // over the weights of step i, scaled an iteration ago
+                ask(i + 3);
+            }
+            if (tid == 0) {
+                bulk_store_read();  // the image before this one has left shared memory: the next may take its place
+                if (i + 2 < count) {  // k of this step, once its product has been made
+                    wait.on(&sh.made[i & 1], (i >> 1) & 1);
+                    load_k(i + 2);
                 }
             }
             tc::fence_async_smem();
-            __syncthreads();
-            if (tid == 0) bulk_store(images + (((long long)c * a.H + h) * g.tiles + tile) * planes * (KP * 128), ws, planes * (KP * 128));
-            float r[32];
-            tc::tmem_ld32(tm + ((unsigned)(32 * (w & 3)) << 16) + c0, r);
-#pragma unroll
-            for (int v = 0; v < 32; ++v) st[v] = fmaf(decay, st[v], r[v]);
             tc::fence_before_sync();
+            __syncthreads();
+            if (tid == 0) {
+                if (more) {
+                    multiply(i + 1);
+                    if (i + 3 < count) load_v(i + 3);
+                }
+                bulk_store(images + (((long long)chunk(i) * a.H + h) * g.tiles + tile) * planes * (KP * 128), to, planes * (KP * 128));
+            }
+            wait.on(&sh.made[i & 1], (i >> 1) & 1);
+            tc::fence_after_sync();
+            const unsigned from = tm + ((unsigned)(32 * (w & 3)) << 16) + 128 * (i & 1) + c0;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float hi[8], lo[8];
+                tmem_ld8x2(from + 8 * q, from + VT + 8 * q, hi, lo);
+#pragma unroll
+                for (int v = 0; v < 8; ++v) st[8 * q + v] = fmaf(decay, st[8 * q + v], hi[v] + lo[v]);
+            }
+            decay = decay1, decay1 = decay2;
+        }
+        if (wait.bad) {
+            atomicCAS(&g_ssm_status, 0, 1);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] = __int_as_float(0x7fc00000);
         }
         if (tid == 0) bulk_store_done();
+        tc::fence_before_sync();
         __syncthreads();
-        if (w == 0) tc::tmem_free(tm, 64);
-    }
-    if (wait.bad) {
-        atomicCAS(&g_ssm_status, 0, 1);
-#pragma unroll
-        for (int v = 0; v < 32; ++v) st[v] = __int_as_float(0x7fc00000);
+        if (w == 0) tc::tmem_free(tm, 256);
     }
     if (end && k < a.K)
 #pragma unroll
-        for (int v = 0; v < 32; ++v)
+        for (int v = 0; v < 16; ++v)
             if (v0 + v < a.V) end[at + (long long)v * a.K] = st[v];
 }
 
@@ -312,6 +369,22 @@ struct __align__(16) Scalars {
 // One token's, asked for a head ahead.
 struct Token {
     float lh, ll, dt, lqh, lql;
+    // gradients: gt of this token as it lies in memory (a conversion would wait for it), the head's bias and g
+    unsigned gt;
+    float bias, g;
+    __device__ __forceinline__ void ask_gt(const SsmArgs& s, const SsmChunk& ch, int h, int t) {
+        const long long at = (ch.tok + min(t, ch.len - 1)) * s.a.H + h;
+        if (s.a.gt_dtype == PALIMPSA_F32) gt = static_cast<const unsigned*>(s.a.gt)[at];
+        else gt = static_cast<const unsigned short*>(s.a.gt)[at];
+        bias = s.a.gt_bias ? s.a.gt_bias[h] : 0.f;
+        g = s.a.g[h];
+    }
+    __device__ __forceinline__ float u(int type) const {
+        const float x = type == PALIMPSA_F32    ? __uint_as_float(gt)
+                        : type == PALIMPSA_BF16 ? __uint_as_float(gt << 16)
+                                                : __half2float(__ushort_as_half((unsigned short)gt));
+        return x + bias;
+    }
     __device__ __forceinline__ void ask(const SsmArgs& s, int c, int h, int t) {
         const long long at = ((long long)c * s.a.H + h) * Q;
         lh = s.lh[at + t], ll = s.ll[at + t], dt = s.dt[at + t];
@@ -328,6 +401,12 @@ struct Token {
 __device__ __forceinline__ void ld4f(const float* p, float (&x)[4]) {
     const float4 y = *reinterpret_cast<const float4*>(p);
     x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+}
+__device__ __forceinline__ void ld8f(const float* p, float (&x)[8]) {
+    float lo[4], hi[4];
+    ld4f(p, lo), ld4f(p + 4, hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
 }
 __device__ __forceinline__ void sync_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // 32 values of row r, columns 32 cb .., into an operand of two boxes.
@@ -346,13 +425,17 @@ __device__ __forceinline__ void zero_tile(char* tile, int bytes, int tid, int nt
 
 // ---- outputs --------------------------------------------------------------------------------------------------------------------------
 // Two groups of 4 warps take the heads and tiles in turn, each with its own P, v, state and accumulators: what one waits for (its
-// tiles, its products), the other fills.  (One group of 8 warps with the same buffers: 4.8 us a head; so: see below.)
-constexpr int THREADS = 256;
+// tiles, its products), the other fills.  (One group of 8 warps with the same buffers: 115 us for 128 chunks of 24 heads, 128x64;
+// so 54.)  At KP = 64 the two are CTAs of their own, two to an SM, whose beginnings overlap as well.
 template <int KP>
-constexpr int out_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * (2 * BOX + BOX + KP * 128) + 2 * (int)sizeof(Scalars); }
+__host__ __device__ constexpr int out_groups() { return KP == 64 ? 1 : 2; }
+template <int KP>
+constexpr int out_smem() {
+    return 1024 + 2 * (KP / 64) * BOX + out_groups<KP>() * (2 * BOX + BOX + KP * 128 + (int)sizeof(Scalars));
+}
 
 template <int KP>
-__global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, const __grid_constant__ CUtensorMap qmap,
+__global__ void __launch_bounds__(Q * out_groups<KP>(), 3 - out_groups<KP>()) ssm_out_tc_kernel(const TcArgs g, const __grid_constant__ CUtensorMap qmap,
                                                              const __grid_constant__ CUtensorMap kmap,
                                                              const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ char raw[];
@@ -362,13 +445,15 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
     const SsmArgs& s = g.s;
     const palimpsa_ssm& a = s.a;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, c = blockIdx.x, hq = blockIdx.y, rep = a.H / a.Hq;
+    constexpr int GROUPS = out_groups<KP>(), TMEM = 128 + 128 * GROUPS > 256 ? 512 : 256;
     const int grp = tid >> 7, t = tid & (Q - 1);  // group, and its thread: row t of the chunk
     char* qt = sm;
     char* kt = qt + (KP / 64) * BOX;
-    char* P = kt + (KP / 64) * BOX + grp * 2 * BOX;
-    char* vt = kt + (KP / 64) * BOX + 4 * BOX + grp * BOX;
-    char* ht = kt + (KP / 64) * BOX + 6 * BOX + grp * KP * 128;
-    Scalars& x = reinterpret_cast<Scalars*>(kt + (KP / 64) * BOX + 6 * BOX + 2 * KP * 128)[grp];
+    char* rest = kt + (KP / 64) * BOX;
+    char* P = rest + grp * 2 * BOX;
+    char* vt = rest + (2 * GROUPS + grp) * BOX;
+    char* ht = rest + 3 * GROUPS * BOX + grp * KP * 128;
+    Scalars& x = reinterpret_cast<Scalars*>(rest + 3 * GROUPS * BOX + GROUPS * KP * 128)[grp];
     const SsmChunk ch = ssm_chunk(s, c);
     if (ch.len == 0) return;
     // this CTA's share of the heads and tiles that read hq
@@ -380,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
         for (int b = 0; b < 2; ++b) tc::mbar_init(&v_loaded[b]), tc::mbar_init(&h_loaded[b]), tc::mbar_init(&made[b]);
         tc::mbar_init_fence();
     }
-    if (w == 0) tc::tmem_alloc(&slot, 512);
+    if (w == 0) tc::tmem_alloc(&slot, TMEM);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -412,28 +497,28 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
     __syncthreads();
     if (ch.len < Q) {
 #pragma unroll
-        for (int b = 0; b < KP / 64; ++b) zero_rows(qt + b * BOX, ch.len, tid, THREADS), zero_rows(kt + b * BOX, ch.len, tid, THREADS);
+        for (int b = 0; b < KP / 64; ++b) zero_rows(qt + b * BOX, ch.len, tid, Q * GROUPS), zero_rows(kt + b * BOX, ch.len, tid, Q * GROUPS);
         tc::fence_async_smem();
         __syncthreads();
     }
     if (tid == 0) {
-        product<false, false>(tS, qt, kt, KP / 16, Q, false);
+        product<false, false, KP / 16, Q>(tS, qt, kt, false);
         tc::commit(&s_made);
     }
     wait.on(&s_made, 0);
     tc::fence_after_sync();
     const int rw = w & 3, r = t;
     const unsigned lanes = (unsigned)(32 * rw) << 16;
-    for (int n = 0; j < j1; ++n, j += 2) {
+    for (int n = 0; j < j1; ++n, j += GROUPS) {
         const int h = hq * rep + j / g.tiles, v0 = (j % g.tiles) * VT;
         next.put(x, t);
         const float lh = next.lh, ll = next.ll, e = x.eL[t];
         sync_group(1 + grp, Q);
-        if (j + 2 < j1) next.ask(s, c, hq * rep + (j + 2) / g.tiles, t);
+        if (j + GROUPS < j1) next.ask(s, c, hq * rep + (j + GROUPS) / g.tiles, t);
         if (t == 0) {
             wait.on(&h_loaded[grp], n & 1);
             tc::fence_after_sync();
-            product<false, true>(tU, qt, ht, KP / 16, VT, false);
+            product<false, true, KP / 16, VT>(tU, qt, ht, false);
         }
         __syncwarp();
 #pragma unroll 1
@@ -470,13 +555,13 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
         sync_group(1 + grp, Q);
         if (t == 0) {
             tc::fence_after_sync();
-            product<false, true>(tY, P, vt, Q / 16, VT, false);
+            product<false, true, Q / 16, VT>(tY, P, vt, false);
             tc::commit(&made[grp]);
         }
         __syncwarp();
         wait.on(&made[grp], n & 1);
         tc::fence_after_sync();
-        if (t == 0 && j + 2 < j1) load_h(j + 2);
+        if (t == 0 && j + GROUPS < j1) load_h(j + GROUPS);
         __syncwarp();
         const float D = a.D ? a.D[h] : 0.f;
 #pragma unroll
@@ -501,22 +586,25 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_out_tc_kernel(const TcArgs g, 
         }
         tc::fence_async_smem();
         sync_group(1 + grp, Q);
-        if (t == 0 && j + 2 < j1) load_v(j + 2);
+        if (t == 0 && j + GROUPS < j1) load_v(j + GROUPS);
         __syncwarp();
     }
     if (wait.bad) atomicCAS(&g_ssm_status, 0, 2);
     tc::fence_before_sync();
     __syncthreads();
-    if (w == 0) tc::tmem_free(tm, 512);
+    if (w == 0) tc::tmem_free(tm, TMEM);
 }
 
 // ---- gradients ------------------------------------------------------------------------------------------------------------------------
+// 16 warps: warp w has rows 32 (w % 4) .. and the block of 32 columns w / 4 (16 columns of a tile of d_v).  (8 warps with two blocks
+// each: 19 500 cycles a head, a quarter of them in the one warp with the longest blocks.)
+constexpr int THREADS = 512;
 struct GradSums {            // of a head, over its tiles
-    float row[2][Q];         // sum_j M_ij over the columns of earlier blocks
+    float row[3][Q];         // sum_j M_ij over the columns of an earlier block
     float col[4][Q];         // sum over the rows of block w of P_ij (do_i.v_j): M_ij / dt_j
     float z[Q];              // sum_{i>=t>j} M_ij inside t's own block
-    float A[2][Q], B[2][Q];  // do_i.(h q_i), v_j.(G k_j), by halves of d_v
-    float dot[8], diag[4];   // <h, G>; do_i.v_i
+    float A[4][Q], B[4][Q];  // do_i.(h q_i), v_j.(G k_j), by quarters of d_v
+    float dot[16], diag[4];  // <h, G>; do_i.v_i
     float cross[4][4], at[4], bt[4], pg[4], pb[4];
 };
 template <int KP>
@@ -577,7 +665,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
         load(h0, 0);
     }
     Token next;
-    if (tid < Q) next.ask(s, c, h0, tid);
+    if (tid < Q) next.ask(s, c, h0, tid), next.ask_gt(s, ch, h0, tid);
     Waits wait;
     zero_tile(P, 2 * BOX, tid, THREADS);
     wait.on(&qk_loaded, 0);
@@ -588,27 +676,25 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
     tc::fence_async_smem();
     __syncthreads();
     if (tid == 0) {
-        product<false, false>(tD, qt, kt, KP / 16, Q, false);
+        product<false, false, KP / 16, Q>(tD, qt, kt, false);
         tc::commit(&inner);
     }
-    const int rw = w & 3, half = w >> 2, r = 32 * rw + lane;
+    const int rw = w & 3, cb = w >> 2, r = 32 * rw + lane;
     const unsigned lanes = (unsigned)(32 * rw) << 16;
-    float S[2][32], dS[2][32];  // of blocks 2 half and 2 half + 1, where they are not above the diagonal
+    float S[32], dS[32], u = 0.f, gh = 0.f;  // the block's, if it is not above the diagonal; the head's gt + bias and g
     wait.on(&inner, 0);
     tc::fence_after_sync();
+    tc::tmem_ld32(tD + lanes + 32 * cb, S);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        tc::tmem_ld32(tD + lanes + 32 * (2 * half + k), S[k]);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) dS[k][i] = 0.f;
-    }
+    for (int i = 0; i < 32; ++i) dS[i] = 0.f;
     tc::fence_before_sync();
     int step = 0;
     for (int h = h0; h < h1; ++h) {
         for (int tile = 0; tile < g.tiles; ++tile, ++step) {
             if (tile == 0 && tid < Q) {
                 next.put(x, tid);
-                if (h + 1 < h1) next.ask(s, c, h + 1, tid);
+                u = next.u(a.gt_dtype), gh = next.g;
+                if (h + 1 < h1) next.ask(s, c, h + 1, tid), next.ask_gt(s, ch, h + 1, tid);
             }
             wait.on(&loaded, step & 1);
             __syncthreads();
@@ -620,14 +706,78 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             }
             if (tid == 0) {
                 tc::fence_after_sync();
-                product<false, false>(tD, dy, vt, VT / 16, Q, false);
+                product<false, false, VT / 16, Q>(tD, dy, vt, false);
                 tc::commit(&inner);
-                product<false, true>(tU, qt, ht, KP / 16, VT, false);
-                product<false, true>(tU, qt, ht + KP * 128, KP / 16, VT, true);
-                product<false, true>(tG, kt, gt, KP / 16, VT, false);
-                product<false, true>(tG, kt, gt + KP * 128, KP / 16, VT, true);
+                products<false, true, KP / 16, VT>(tU, qt, ht, tG, kt, gt, false);
+                products<false, true, KP / 16, VT>(tU, qt, ht + KP * 128, tG, kt, gt + KP * 128, true);
             }
             auto put = [tile](float& to, float y) { to = tile ? to + y : y; };
+            wait.on(&inner, (step + 1) & 1);
+            tc::fence_after_sync();
+            if (cb <= rw) {
+                const float lh = x.lh[r], ll = x.ll[r];
+                float t[32];
+                tc::tmem_ld32(tD + lanes + 32 * cb, t);
+                if (cb < rw) {
+                    const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
+                    float early = 0.f;
+#pragma unroll
+                    for (int i0 = 0; i0 < 32; i0 += 8) {
+                        float b8[8], d8[8], p[8];
+                        ld8f(x.bl + 32 * cb + i0, b8), ld8f(x.dt + 32 * cb + i0, d8);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int i = i0 + e;
+                            const float dec = ai * b8[e], q = t[i] * dec;
+                            p[e] = S[i] * dec;
+                            t[i] = q * S[i];
+                            dS[i] = fmaf(q, d8[e], dS[i]);
+                            early = fmaf(t[i], d8[e], early);
+                        }
+                        *chunk_at(P + (cb >> 1) * BOX, r, (cb & 1) * 4 + i0 / 8) = pack8_finite(p);
+                    }
+                    put(sums.row[cb][r], early);
+                } else {
+                    float diag = 0.f;
+#pragma unroll
+                    for (int i0 = 0; i0 < 32; i0 += 8) {
+                        float h8[8], l8[8], d8[8], p[8];
+                        ld8f(x.lh + 32 * cb + i0, h8), ld8f(x.ll + 32 * cb + i0, l8), ld8f(x.dt + 32 * cb + i0, d8);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int i = i0 + e;
+                            const float dec = i <= lane ? ex2(((lh - h8[e]) + (ll - l8[e])) * LOG2E) : 0.f;
+                            const float q = i <= lane ? t[i] * dec : 0.f;
+                            if (i == lane) diag = t[i];
+                            p[e] = i <= lane ? S[i] * dec : 0.f;
+                            t[i] = q * S[i];
+                            dS[i] = fmaf(q, d8[e], dS[i]);
+                        }
+                        *chunk_at(P + (cb >> 1) * BOX, r, (cb & 1) * 4 + i0 / 8) = pack8_finite(p);
+                    }
+                    // row i brings sum_{j<t} M_ij to the borders t <= i
+                    float p[32], run = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        p[i] = i <= lane ? run : 0.f;
+                        run = fmaf(t[i], x.dt[32 * cb + i], run);
+                    }
+                    xreduce<32, 32>(p, lane);
+                    put(sums.z[32 * cb + xreduce_index<32, 32>(lane)], p[0]);
+                    diag = warp_add(diag);
+                    if (lane == 0) put(sums.diag[cb], diag);
+                }
+                xreduce<32, 32>(t, lane);
+                put(sums.col[rw][32 * cb + xreduce_index<32, 32>(lane)], t[0]);
+            }
+            tc::fence_async_smem();
+            tc::fence_before_sync();
+            __syncthreads();
+            if (tid == 0) {
+                tc::fence_after_sync();
+                product<true, true, Q / 16, VT>(tD, P, dy, false);
+                tc::commit(&pv);
+            }
             {   // <h, G>
                 float d = 0.f;
                 for (int i = tid; i < KP * 8; i += THREADS) {
@@ -642,84 +792,15 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 d = warp_add(d);
                 if (lane == 0) put(sums.dot[w], d);
             }
-            wait.on(&inner, (step + 1) & 1);
-            tc::fence_after_sync();
-            float early = 0.f;
-            const float lh = x.lh[r], ll = x.ll[r];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int cb = 2 * half + k;
-                if (cb > rw) break;
-                float t[32], p[32];
-                tc::tmem_ld32(tD + lanes + 32 * cb, t);
-                if (cb < rw) {
-                    const float ai = ex2(((lh - x.lh[32 * cb + 31]) + (ll - x.ll[32 * cb + 31])) * LOG2E);
-#pragma unroll
-                    for (int i0 = 0; i0 < 32; i0 += 4) {
-                        float b4[4], d4[4];
-                        ld4f(x.bl + 32 * cb + i0, b4), ld4f(x.dt + 32 * cb + i0, d4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = i0 + e;
-                            const float dec = ai * b4[e], q = t[i] * dec;
-                            p[i] = S[k][i] * dec;
-                            t[i] = q * S[k][i];
-                            dS[k][i] = fmaf(q, d4[e], dS[k][i]);
-                            early = fmaf(t[i], d4[e], early);
-                        }
-                    }
-                    st_block(P, r, cb, p);
-                } else {
-                    float diag = 0.f;
-#pragma unroll
-                    for (int i0 = 0; i0 < 32; i0 += 4) {
-                        float h4[4], l4[4], d4[4];
-                        ld4f(x.lh + 32 * cb + i0, h4), ld4f(x.ll + 32 * cb + i0, l4), ld4f(x.dt + 32 * cb + i0, d4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = i0 + e;
-                            const float dec = i <= lane ? ex2(((lh - h4[e]) + (ll - l4[e])) * LOG2E) : 0.f;
-                            const float q = i <= lane ? t[i] * dec : 0.f;
-                            if (i == lane) diag = t[i];
-                            p[i] = i <= lane ? S[k][i] * dec : 0.f;
-                            t[i] = q * S[k][i];
-                            dS[k][i] = fmaf(q, d4[e], dS[k][i]);
-                        }
-                    }
-                    st_block(P, r, cb, p);
-                    // row i brings sum_{j<t} M_ij to the borders t <= i
-                    float run = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        p[i] = i <= lane ? run : 0.f;
-                        run = fmaf(t[i], x.dt[32 * cb + i], run);
-                    }
-                    xreduce<32, 32>(p, lane);
-                    put(sums.z[32 * cb + xreduce_index<32, 32>(lane)], p[0]);
-                    diag = warp_add(diag);
-                    if (lane == 0) put(sums.diag[cb], diag);
-                }
-                xreduce<32, 32>(t, lane);
-                put(sums.col[rw][32 * cb + xreduce_index<32, 32>(lane)], t[0]);
-            }
-            put(sums.row[half][r], early);
-            tc::fence_async_smem();
-            tc::fence_before_sync();
-            __syncthreads();
-            if (tid == 0) {
-                tc::fence_after_sync();
-                product<true, true>(tD, P, dy, Q / 16, VT, false);
-                tc::commit(&pv);
-            }
             wait.on(&pv, step & 1);
             tc::fence_after_sync();
-            {   // row r of all three, 32 columns: dv, and what do and v become as operands of dq and dk
+            {   // row r of all three, 16 columns: dv, and what do and v become as operands of dq and dk
                 float A = 0.f, B = 0.f;
                 const float dt = x.dt[r], wq = x.wq[r], eL = x.eL[r], wd = wq * dt, D = a.D ? a.D[h] : 0.f;
                 char* out = P + (r < 96 ? (32 + r) * 128 : BOX + r * 128);  // rows of P that every head writes anew
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int cc = 4 * half + q;
+                for (int q = 0; q < 2; ++q) {
+                    const int cc = 2 * cb + q;
                     float u1[8], u2[8], pd[8], v[8], d[8];
                     tmem_ld8x3(tU + lanes + 8 * cc, tG + lanes + 8 * cc, tD + lanes + 8 * cc, u1, u2, pd);
                     unpack8(*chunk_at(vt, r, cc), v);
@@ -737,16 +818,15 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                     *chunk_at(vt, r, cc) = pack8(v);
                     *chunk_at(dy, r, cc) = pack8(d);
                 }
-                put(sums.A[half][r], A);
-                put(sums.B[half][r], B);
+                put(sums.A[cb][r], A);
+                put(sums.B[cb][r], B);
             }
             tc::fence_async_smem();
             tc::fence_before_sync();
             __syncthreads();
             if (tid == 0) {
                 tc::fence_after_sync();
-                product<false, false>(tQ, dy, ht, VT / 16, KP, step > 0);
-                product<false, false>(tK, vt, gt, VT / 16, KP, step > 0);
+                products<false, false, VT / 16, KP>(tQ, dy, ht, tK, vt, gt, step > 0);
                 tc::commit(&outer);
             }
             const int v0 = tile * VT;
@@ -771,8 +851,8 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 float ta = 0.f, tb = 0.f, late = 0.f, own = 0.f, direct = 0.f, dt = 0.f;
                 if (tid < Q) {
                     dt = x.dt[t];
-                    ta = x.eL[t] * (sums.A[0][t] + sums.A[1][t]);
-                    own = x.wq[t] * (sums.B[0][t] + sums.B[1][t]);
+                    ta = x.eL[t] * ((sums.A[0][t] + sums.A[1][t]) + (sums.A[2][t] + sums.A[3][t]));
+                    own = x.wq[t] * ((sums.B[0][t] + sums.B[1][t]) + (sums.B[2][t] + sums.B[3][t]));
                     tb = dt * own;
                     direct = sums.col[b][t];
                     for (int k = b + 1; k < 4; ++k) {
@@ -787,7 +867,8 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 }
                 __syncthreads();
                 if (tid < Q) {
-                    float suf = sums.row[0][t] + sums.row[1][t] + ta, pre = late + tb;
+                    float suf = ta, pre = late + tb;
+                    for (int k = 0; k < b; ++k) suf += sums.row[k][t];
 #pragma unroll
                     for (int d = 1; d < 32; d *= 2) {
                         const float y = __shfl_down_sync(0xffffffffu, suf, d), u = __shfl_up_sync(0xffffffffu, pre, d);
@@ -801,14 +882,13 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                     for (int k = b + 1; k < 4; ++k)
                         for (int i = 0; i < b; ++i) dlf += sums.cross[k][i];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) hG += sums.dot[k];
+                    for (int k = 0; k < 16; ++k) hG += sums.dot[k];
                     dlf = fmaf(x.eL[Q - 1], hG, dlf);
-                    float ddt = direct + own - a.g[h] * dlf;
+                    float ddt = direct + own - gh * dlf;
                     float pg = 0.f, pb = 0.f;
                     if (wait.bad) ddt = dlf = __int_as_float(0x7fc00000);
                     if (t < ch.len) {
                         const long long at = (ch.tok + t) * a.H + h;
-                        const float u = ld_any(a.gt, at, a.gt_dtype) + (a.gt_bias ? a.gt_bias[h] : 0.f);
                         ddt *= ssm_ddt(u, (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0);
                         st1(a.dgt, at, ddt, a.gt_dtype);
                         pg = -dt * dlf, pb = ddt;
@@ -828,28 +908,27 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
         }
     }
     // dq += dS k, dk += dS^T q
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        if (2 * half + k <= rw) st_block(P, r, 2 * half + k, dS[k]);
+    if (cb <= rw) st_block(P, r, cb, dS);
     tc::fence_async_smem();
     tc::fence_before_sync();
     __syncthreads();
     if (tid == 0) {
         tc::fence_after_sync();
-        product<false, true>(tQ, P, kt, Q / 16, KP, true);
-        product<true, true>(tK, P, qt, Q / 16, KP, true);
+        product<false, true, Q / 16, KP>(tQ, P, kt, true);
+        product<true, true, Q / 16, KP>(tK, P, qt, true);
         tc::commit(&outer);
     }
     wait.on(&outer, step & 1);
     tc::fence_after_sync();
-    // dq by the first four warps, dk by the others: a row each, 8 columns a time
+    // dq by the first eight warps, dk by the others: half a row each, 16 columns a time
     {
+        const int half = cb >> 1;
         const unsigned from = (half ? tK : tQ) + lanes;
         const long long row = (ch.tok + r) * a.Hq + hq;
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(half ? a.dk : a.dq) + row * a.K;
         float* part = g.splits > 1 ? g.part_qk + (((long long)half * g.splits + blockIdx.z) * a.total_tokens * a.Hq + row) * a.K : nullptr;
 #pragma unroll 1
-        for (int k0 = 0; k0 < KP; k0 += 16) {
+        for (int k0 = (cb & 1) * (KP / 2); k0 < (cb & 1) * (KP / 2) + KP / 2; k0 += 16) {
             float y[8], z[8];
             tmem_ld8x2(from + k0, from + k0 + 8, y, z);
             if (wait.bad) y[0] = z[0] = __int_as_float(0x7fc00000);
@@ -921,18 +1000,18 @@ int launched() { return cudaGetLastError() == cudaSuccess ? PALIMPSA_OK : PALIMP
 
 // Into how many shares a chunk's heads (times tiles where `tiles` of them may be parted) go: whole waves of CTAs times what one
 // takes, with `fixed` steps for what a CTA does once.
-int shares(long long ctas, int steps, double fixed) {
+int shares(long long ctas, int steps, double fixed, int resident) {
     int best = 1;
     double least = 1e30;
     for (int n = 1; n <= steps; ++n) {
         const int per = (steps + n - 1) / n;
         if ((steps + per - 1) / per != n) continue;  // the same shares as a smaller n, some empty
-        const double cost = (double)((ctas * n + B200_SMS - 1) / B200_SMS) * (per + fixed);
+        const double cost = (double)((ctas * n + resident - 1) / resident) * (per + fixed);
         if (cost < least * 0.97) least = cost, best = n;
     }
     return best;
 }
-int grad_shares(const palimpsa_ssm& a, long long chunks) { return shares(chunks * a.Hq, a.H / a.Hq, 1.5 / tiles_of(a)); }
+int grad_shares(const palimpsa_ssm& a, long long chunks) { return shares(chunks * a.Hq, a.H / a.Hq, 1.5 / tiles_of(a), B200_SMS); }
 
 TcArgs tc_args(const SsmArgs& s, bool training) {
     TcArgs g{};
@@ -978,14 +1057,16 @@ int ssm_tc_fwd(const SsmArgs& s, bool training, cudaStream_t st) {
     if (a.num_seqs > 0)
         if (int rc = wide ? launch_walk<128, false>(g, k, v, st) : launch_walk<64, false>(g, k, v, st)) return rc;
     if (s.chunks == 0) return PALIMPSA_OK;
-    g.splits = shares((long long)s.chunks * a.Hq, a.H / a.Hq * g.tiles, 2.);
+    // a CTA's beginning costs about as much as two heads
+    g.splits = wide ? shares((long long)s.chunks * a.Hq, a.H / a.Hq * g.tiles, 2., B200_SMS)
+                    : shares((long long)s.chunks * a.Hq, a.H / a.Hq * g.tiles, 2., 2 * B200_SMS);
     const dim3 grid(s.chunks, a.Hq, g.splits);
     if (wide) {
         if (!allow_smem<ssm_out_tc_kernel<128>>(out_smem<128>())) return PALIMPSA_E_LAUNCH;
-        ssm_out_tc_kernel<128><<<grid, THREADS, out_smem<128>(), st>>>(g, q, k, v);
+        ssm_out_tc_kernel<128><<<grid, Q * out_groups<128>(), out_smem<128>(), st>>>(g, q, k, v);
     } else {
         if (!allow_smem<ssm_out_tc_kernel<64>>(out_smem<64>())) return PALIMPSA_E_LAUNCH;
-        ssm_out_tc_kernel<64><<<grid, THREADS, out_smem<64>(), st>>>(g, q, k, v);
+        ssm_out_tc_kernel<64><<<grid, Q * out_groups<64>(), out_smem<64>(), st>>>(g, q, k, v);
     }
     return launched();
 }
