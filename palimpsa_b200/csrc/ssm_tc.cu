@@ -16,7 +16,8 @@
 // gradients of dt, g and D -- takes both parts of its operand (2^-17), and S and do v^T of the decays' gradients stay float32.
 //
 // Rows of a tile behind a sequence's end are other tokens' or fill; they are zeroed in shared memory, so that whatever they hold
-// never meets a zero weight as NaN.  Every wait is bounded: one that gives up sets g_ssm_status and its CTA's outputs become NaN.
+// never meets a zero weight as NaN.  Every wait is bounded: one that gives up sets g_ssm_status, and what its CTA writes last (states, outputs,
+// gradients) becomes NaN.
 #include "ssm.cuh"
 #include "tc_common.cuh"
 
@@ -163,17 +164,18 @@ struct Waits {
 // step i is written out, so that a step costs its CUDA-core work and one barrier.  Everything a step writes has two buffers; k and
 // v are asked for one and two steps ahead.  (One step after the other, two CTAs an SM: 66 us for 192 walks of 16 steps, 69 for 64 of
 // 24; so: see ssm_tc_fwd.)
-constexpr int WALK_THREADS = 512;  // thread: row k = tid % 128 of the state, 16 columns of d_v by tid / 128
+constexpr int WALK_THREADS = 512;  // and a warp that issues products and copies (3000 cycles a step, if a warp does it beside its share);
+                                   // thread: row k = tid % 128 of the state, 16 columns of d_v by tid / 128
 struct WalkShared {
     float w[2][Q];
     unsigned long long k_loaded[2], v_loaded[2], made[2];
-    unsigned slot;
+    unsigned slot, failed;
 };
 template <int KP>
 constexpr int walk_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * BOX + 4 * BOX + 4 * KP * 128 + (int)sizeof(WalkShared); }
 
 template <int KP, bool BACKWARD>
-__global__ void __launch_bounds__(WALK_THREADS, 1) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
                                                                 const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ char raw[];
     char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
@@ -192,13 +194,15 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) ssm_walk_kernel(const TcArgs 
     float* end = BACKWARD ? a.dh0 : a.h_out;
     const int planes = BACKWARD ? 2 : g.planes;
     char* images = BACKWARD ? g.grad : g.state;
-    const int k = tid & (Q - 1), c0 = (tid >> 7) * 16, v0 = tile * VT + c0;
+    const bool issuer = tid >= WALK_THREADS;  // its lane 0
+    const int k = issuer ? a.K : tid & (Q - 1), c0 = (tid >> 7) * 16, v0 = tile * VT + c0;
     const long long at = ((long long)nh * a.V + v0) * a.K + k;
     float st[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) st[v] = start && k < a.K && v0 + v < a.V ? start[at + (long long)v * a.K] : 0.f;
     if (count > 0) {
         if (tid == 0) {
+            sh.failed = 0;
             for (int b = 0; b < 2; ++b) tc::mbar_init(&sh.k_loaded[b]), tc::mbar_init(&sh.v_loaded[b]), tc::mbar_init(&sh.made[b]);
             tc::mbar_init_fence();
             tc::tma_prefetch_map(&kmap);
@@ -276,83 +280,96 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) ssm_walk_kernel(const TcArgs 
             product<true, true, Q / 16, 2 * VT>(tm + 128 * (i & 1), kb, wb, false);  // both parts: 64 columns each
             tc::commit(&sh.made[i & 1]);
         };
-        if (tid == 0) {
-            for (int i = 0; i < 2 && i < count; ++i) load_v(i), load_k(i);
-        }
-        ask(0);
-        float decay = put(0), decay1 = 1.f;
-        ask(1);
-        if (count > 1) decay1 = put(1);
-        ask(2);
-        __syncthreads();
-        scale(0, ssm_chunk(s, chunk(0)).len);
-        tc::fence_async_smem();
-        tc::fence_before_sync();
-        __syncthreads();
-        if (tid == 0) {
-            multiply(0);
-            if (count > 2) load_v(2);
-        }
-        for (int i = 0; i < count; ++i) {
-            const bool more = i + 1 < count;
-            if (more) scale(i + 1, ssm_chunk(s, chunk(i + 1)).len);
-            // the image of the state in front of (behind) this chunk: row k, 16 columns
-            char* to = img + (i & 1) * 2 * KP * 128;
-            if (k < KP) {
-#pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    float hi[8], lo[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        hi[e] = __bfloat162float(__float2bfloat16_rn(st[8 * cc + e]));
-                        lo[e] = st[8 * cc + e] - hi[e];
+        if (issuer) {
+            const bool one = tid == WALK_THREADS;
+            if (one)
+                for (int i = 0; i < 2 && i < count; ++i) load_v(i), load_k(i);
+            __syncwarp();
+            __syncthreads();  // the first weights
+            __syncthreads();  // the first operand
+            if (one) {
+                multiply(0);
+                if (count > 2) load_v(2);
+            }
+            __syncwarp();
+            for (int i = 0; i < count; ++i) {
+                if (one) {
+                    bulk_store_read();  // the image of the step before has left shared memory: the next may take its place
+                    if (i + 2 < count) {  // k of this step, once its product has been made
+                        wait.on(&sh.made[i & 1], (i >> 1) & 1);
+                        load_k(i + 2);
                     }
-                    *chunk_at(to, k, c0 / 8 + cc) = pack8(hi);
-                    if (planes == 2) *chunk_at(to + KP * 128, k, c0 / 8 + cc) = pack8(lo);
                 }
-            }
-            float decay2 = 1.f;
-            if (i + 2 < count) {
-                decay2 = put(i + 2);  // over the weights of step i, scaled an iteration ago
-                ask(i + 3);
-            }
-            if (tid == 0) {
-                bulk_store_read();  // the image before this one has left shared memory: the next may take its place
-                if (i + 2 < count) {  // k of this step, once its product has been made
-                    wait.on(&sh.made[i & 1], (i >> 1) & 1);
-                    load_k(i + 2);
+                __syncwarp();
+                __syncthreads();  // operand i + 1 and image i are there
+                if (one) {
+                    if (i + 1 < count) multiply(i + 1);
+                    bulk_store(images + (((long long)chunk(i) * a.H + h) * g.tiles + tile) * planes * (KP * 128), img + (i & 1) * 2 * KP * 128,
+                               planes * (KP * 128));
+                    if (i + 3 < count) load_v(i + 3);
                 }
+                __syncwarp();
             }
+            if (one) bulk_store_done();
+        } else {
+            ask(0);
+            float decay = put(0), decay1 = 1.f;
+            ask(1);
+            if (count > 1) decay1 = put(1);
+            ask(2);
+            __syncthreads();
+            scale(0, ssm_chunk(s, chunk(0)).len);
             tc::fence_async_smem();
             tc::fence_before_sync();
             __syncthreads();
-            if (tid == 0) {
-                if (more) {
-                    multiply(i + 1);
-                    if (i + 3 < count) load_v(i + 3);
+            for (int i = 0; i < count; ++i) {
+                if (i + 1 < count) scale(i + 1, ssm_chunk(s, chunk(i + 1)).len);
+                // the image of the state in front of (behind) this chunk: row k, 16 columns
+                char* to = img + (i & 1) * 2 * KP * 128;
+                if (k < KP) {
+#pragma unroll
+                    for (int cc = 0; cc < 2; ++cc) {
+                        float hi[8], lo[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            hi[e] = __bfloat162float(__float2bfloat16_rn(st[8 * cc + e]));
+                            lo[e] = st[8 * cc + e] - hi[e];
+                        }
+                        *chunk_at(to, k, c0 / 8 + cc) = pack8(hi);
+                        if (planes == 2) *chunk_at(to + KP * 128, k, c0 / 8 + cc) = pack8(lo);
+                    }
                 }
-                bulk_store(images + (((long long)chunk(i) * a.H + h) * g.tiles + tile) * planes * (KP * 128), to, planes * (KP * 128));
-            }
-            wait.on(&sh.made[i & 1], (i >> 1) & 1);
-            tc::fence_after_sync();
-            const unsigned from = tm + ((unsigned)(32 * (w & 3)) << 16) + 128 * (i & 1) + c0;
+                float decay2 = 1.f;
+                if (i + 2 < count) {
+                    decay2 = put(i + 2);  // over the weights of step i, scaled an iteration ago
+                    ask(i + 3);
+                }
+                tc::fence_async_smem();
+                tc::fence_before_sync();
+                __syncthreads();
+                wait.on(&sh.made[i & 1], (i >> 1) & 1);
+                tc::fence_after_sync();
+                const unsigned from = tm + ((unsigned)(32 * (w & 3)) << 16) + 128 * (i & 1) + c0;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float hi[8], lo[8];
-                tmem_ld8x2(from + 8 * q, from + VT + 8 * q, hi, lo);
+                for (int q = 0; q < 2; ++q) {
+                    float hi[8], lo[8];
+                    tmem_ld8x2(from + 8 * q, from + VT + 8 * q, hi, lo);
 #pragma unroll
-                for (int v = 0; v < 8; ++v) st[8 * q + v] = fmaf(decay, st[8 * q + v], hi[v] + lo[v]);
+                    for (int v = 0; v < 8; ++v) st[8 * q + v] = fmaf(decay, st[8 * q + v], hi[v] + lo[v]);
+                }
+                decay = decay1, decay1 = decay2;
             }
-            decay = decay1, decay1 = decay2;
         }
         if (wait.bad) {
             atomicCAS(&g_ssm_status, 0, 1);
+            sh.failed = 1;
+        }
+        tc::fence_before_sync();
+        __syncthreads();
+        if (sh.failed) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) st[v] = __int_as_float(0x7fc00000);
         }
-        if (tid == 0) bulk_store_done();
-        tc::fence_before_sync();
-        __syncthreads();
         if (w == 0) tc::tmem_free(tm, 256);
     }
     if (end && k < a.K)
@@ -599,6 +616,7 @@ __global__ void __launch_bounds__(Q * out_groups<KP>(), 3 - out_groups<KP>()) ss
 // 16 warps: warp w has rows 32 (w % 4) .. and the block of 32 columns w / 4 (16 columns of a tile of d_v).  (8 warps with two blocks
 // each: 19 500 cycles a head, a quarter of them in the one warp with the longest blocks.)
 constexpr int THREADS = 512;
+constexpr int ISSUER = 384;  // issues products and loads: of warp 12, whose block lies above the diagonal, so that it has time
 struct GradSums {            // of a head, over its tiles
     float row[3][Q];         // sum_j M_ij over the columns of an earlier block
     float col[4][Q];         // sum over the rows of block w of P_ij (do_i.v_j): M_ij / dt_j
@@ -655,7 +673,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
         bulk_load(ht, g.state + at, 2 * KP * 128, &loaded);
         bulk_load(gt, g.grad + at, 2 * KP * 128, &loaded);
     };
-    if (tid == 0) {
+    if (tid == ISSUER) {
         tc::mbar_expect_tx(&qk_loaded, 2 * (KP / 64) * BOX);
 #pragma unroll
         for (int b = 0; b < KP / 64; ++b) {
@@ -675,7 +693,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
         for (int b = 0; b < KP / 64; ++b) zero_rows(qt + b * BOX, ch.len, tid, THREADS), zero_rows(kt + b * BOX, ch.len, tid, THREADS);
     tc::fence_async_smem();
     __syncthreads();
-    if (tid == 0) {
+    if (tid == ISSUER) {
         product<false, false, KP / 16, Q>(tD, qt, kt, false);
         tc::commit(&inner);
     }
@@ -704,7 +722,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 tc::fence_async_smem();
                 __syncthreads();
             }
-            if (tid == 0) {
+            if (tid == ISSUER) {
                 tc::fence_after_sync();
                 product<false, false, VT / 16, Q>(tD, dy, vt, false);
                 tc::commit(&inner);
@@ -773,7 +791,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             tc::fence_async_smem();
             tc::fence_before_sync();
             __syncthreads();
-            if (tid == 0) {
+            if (tid == ISSUER) {
                 tc::fence_after_sync();
                 product<true, true, Q / 16, VT>(tD, P, dy, false);
                 tc::commit(&pv);
@@ -824,7 +842,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             tc::fence_async_smem();
             tc::fence_before_sync();
             __syncthreads();
-            if (tid == 0) {
+            if (tid == ISSUER) {
                 tc::fence_after_sync();
                 products<false, false, VT / 16, KP>(tQ, dy, ht, tK, vt, gt, step > 0);
                 tc::commit(&outer);
@@ -842,7 +860,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             tc::fence_after_sync();
             tc::fence_async_smem();
             __syncthreads();  // the tiles, and P behind dv, may be written again
-            if (tid == 0) {
+            if (tid == ISSUER) {
                 if (tile + 1 < g.tiles) load(h, tile + 1);
                 else if (h + 1 < h1) load(h + 1, 0);
             }
@@ -912,7 +930,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
     tc::fence_async_smem();
     tc::fence_before_sync();
     __syncthreads();
-    if (tid == 0) {
+    if (tid == ISSUER) {
         tc::fence_after_sync();
         product<false, true, Q / 16, KP>(tQ, P, kt, true);
         product<true, true, Q / 16, KP>(tK, P, qt, true);
@@ -1040,7 +1058,7 @@ template <int KP, bool BACKWARD>
 static int launch_walk(const TcArgs& g, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
     const palimpsa_ssm& a = g.s.a;
     if (!allow_smem<ssm_walk_kernel<KP, BACKWARD>>(walk_smem<KP>())) return PALIMPSA_E_LAUNCH;
-    ssm_walk_kernel<KP, BACKWARD><<<dim3(a.num_seqs * a.H, g.tiles), WALK_THREADS, walk_smem<KP>(), st>>>(g, kmap, vmap);
+    ssm_walk_kernel<KP, BACKWARD><<<dim3(a.num_seqs * a.H, g.tiles), WALK_THREADS + 32, walk_smem<KP>(), st>>>(g, kmap, vmap);
     return launched();
 }
 
