@@ -142,6 +142,46 @@ def test_long_sequence_of_slow_decays(dtype):
     check(d, got, False)
 
 
+@pytest.mark.parametrize("dtype,K,V", [(torch.float32, 16, 24), (torch.bfloat16, 64, 64), (torch.bfloat16, 128, 96)])
+def test_what_one_sequence_holds_stays_in_it(dtype, K, V):
+    """NaN and infinities in one sequence of a batch, packed or not: the others come out, forward and backward, as without them."""
+    cu = [0, 70, 200, 330]
+    d = make(16, 1, 330, 2, 1, K, V, dtype, n=3)
+    clean = run(d, True, cu=cu)
+    for n, bad in (("q", float("nan")), ("k", float("inf")), ("v", float("nan")), ("do", float("inf")), ("gt", float("nan"))):
+        e = {m: None if t is None else t.clone() for m, t in d.items()}
+        e[n][0, 70:200] = bad
+        got = run(e, True, cu=cu)
+        for m in ("o", "dq", "dk", "dv", "dgt"):
+            for a, b in ((0, 70), (200, 330)):
+                assert torch.equal(got[m][0, a:b], clean[m][0, a:b]), (n, m)
+        for m in ("h", "dh0"):
+            assert torch.equal(got[m][[0, 2]], clean[m][[0, 2]]), (n, m)
+    batch = make(17, 3, 130, 2, 1, K, V, dtype)
+    clean = run(batch, True)
+    for n in ("q", "k", "v", "do"):
+        e = {m: None if t is None else t.clone() for m, t in batch.items()}
+        e[n][1] = float("nan")
+        got = run(e, True)
+        for m in ("o", "dq", "dk", "dv", "dgt", "h", "dh0"):
+            assert torch.equal(got[m][[0, 2]], clean[m][[0, 2]]), (n, m)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_through_the_final_state_alone(dtype):
+    from palimpsa_b200.ops import chunk_ssm
+    d = make(18, 2, 128, 2, 1, 64, 64, dtype)
+    x = on_gpu(d)
+    _, h = chunk_ssm(x["q"], x["k"], x["v"], x["gt"], x["g"], gt_softplus=True, initial_state=x["h0"], output_final_state=True)
+    got = torch.autograd.grad(h, [x["v"], x["h0"], x["q"]], x["dh"])
+    assert not got[2].any()
+    kw = dict(softplus=True, h0=d["h0"], do=torch.zeros_like(d["do"]), dh=d["dh"])
+    ref, mag = (bo.ssm(d["q"], d["k"], d["v"], d["gt"], d["g"], magnitude=m, **kw) for m in (False, True))
+    for name, y in (("dv", got[0]), ("dh0", got[1])):
+        inner = 600 * 2.0 ** -24 + (4 * 2.0 ** -16 if dtype == torch.bfloat16 else 0)
+        assert ((y.cpu().double() - ref[name]).abs() <= inner * mag[name] + HALF[y.dtype] * ref[name].abs() + 1e-30).all()
+
+
 def test_rows_apart_are_read_in_place_and_copied_where_they_must_be():
     from palimpsa_b200.ops import chunk_ssm
     for dtype, T in ((torch.float32, 37), (torch.bfloat16, 140)):
