@@ -160,6 +160,7 @@ struct Waits {
 };
 
 // ---- states, and backwards their gradients, in front of (behind) every chunk ------------------------------------------------------
+// w v is taken in three parts (24 bits), so that the states are those of float32: 1e-7, with two parts 2e-6.
 // Steps are pipelined: while the product of step i runs, the operand of step i+1 is scaled and the image of the state in front of
 // step i is written out, so that a step costs its CUDA-core work and one barrier.  Everything a step writes has two buffers; k and
 // v are asked for one and two steps ahead.  (One step after the other, two CTAs an SM: 66 us for 192 walks of 16 steps, 69 for 64 of
@@ -168,11 +169,11 @@ constexpr int WALK_THREADS = 512;  // and a warp that issues products and copies
                                    // thread: row k = tid % 128 of the state, 16 columns of d_v by tid / 128
 struct WalkShared {
     float w[2][Q];
-    unsigned long long k_loaded[2], v_loaded[2], made[2];
+    unsigned long long k_loaded[2], v_loaded[2], made[2], img_free;
     unsigned slot, failed;
 };
 template <int KP>
-constexpr int walk_smem() { return 1024 + 2 * (KP / 64) * BOX + 2 * BOX + 4 * BOX + 4 * KP * 128 + (int)sizeof(WalkShared); }
+constexpr int walk_smem() { return 1024 + 2 * (KP / 64) * BOX + 6 * BOX + 2 * BOX + 2 * KP * 128 + (int)sizeof(WalkShared); }
 
 template <int KP, bool BACKWARD>
 __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const TcArgs g, const __grid_constant__ CUtensorMap kmap,
@@ -181,9 +182,9 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
     char* sm = raw + ((1024u - (tc::smem_u32(raw) & 1023u)) & 1023u);
     char* kt = sm;                          // k (backwards q): two buffers of KP/64 boxes (KP = 64: the product's rows 64.. are of
     char* ws = kt + 2 * (KP / 64) * BOX;    // what lies behind the box, and not read)
-    char* vt = ws + 4 * BOX;                // ws: w v in two parts, twice
-    char* img = vt + 2 * BOX;               // the state's image in two parts, twice
-    WalkShared& sh = *reinterpret_cast<WalkShared*>(img + 4 * KP * 128);
+    char* vt = ws + 6 * BOX;                // ws: w v in three parts, twice
+    char* img = vt + 2 * BOX;               // the state's image in two parts
+    WalkShared& sh = *reinterpret_cast<WalkShared*>(img + 2 * KP * 128);
     const SsmArgs& s = g.s;
     const palimpsa_ssm& a = s.a;
     const int tid = threadIdx.x, w = tid >> 5, tile = blockIdx.y, nh = blockIdx.x, n = nh / a.H, h = nh - n * a.H, hq = h / (a.H / a.Hq);
@@ -204,11 +205,12 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
         if (tid == 0) {
             sh.failed = 0;
             for (int b = 0; b < 2; ++b) tc::mbar_init(&sh.k_loaded[b]), tc::mbar_init(&sh.v_loaded[b]), tc::mbar_init(&sh.made[b]);
+            tc::mbar_init(&sh.img_free);
             tc::mbar_init_fence();
             tc::tma_prefetch_map(&kmap);
             tc::tma_prefetch_map(&vmap);
         }
-        if (w == 0) tc::tmem_alloc(&sh.slot, 256);
+        if (w == 0) tc::tmem_alloc(&sh.slot, 512);
         tc::fence_before_sync();
         __syncthreads();
         tc::fence_after_sync();
@@ -242,14 +244,14 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
             if (tid < Q) sh.w[i & 1][tid] = BACKWARD ? expf(l0 + l1) : expf((lq0 - l0) + (lq1 - l1)) * dt;
             return expf(lq0 + lq1);
         };
-        auto scale = [&](int i, int len) {  // w v in two parts: row = token, 8 columns a time
+        auto scale = [&](int i, int len) {  // w v in three parts: row = token, 8 columns a time
             wait.on(&sh.v_loaded[i & 1], (i >> 1) & 1);
             char* from = vt + (i & 1) * BOX;
-            char* to = ws + (i & 1) * 2 * BOX;
+            char* to = ws + (i & 1) * 3 * BOX;
 #pragma unroll
             for (int j = 0; j < Q * 8 / WALK_THREADS; ++j) {
                 const int r = (tid >> 3) + j * (WALK_THREADS / 8), cc = tid & 7;
-                float x[8], hi[8], lo[8];
+                float x[8], hi[8], mid[8], lo[8];
                 if (r < len) {
                     unpack8(*chunk_at(from, r, cc), x);
                     const float f = sh.w[i & 1][r];
@@ -257,14 +259,16 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
                     for (int e = 0; e < 8; ++e) {
                         const float y = x[e] * f;
                         hi[e] = __bfloat162float(__float2bfloat16_rn(y));
-                        lo[e] = y - hi[e];
+                        mid[e] = __bfloat162float(__float2bfloat16_rn(y - hi[e]));
+                        lo[e] = y - hi[e] - mid[e];
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) hi[e] = lo[e] = 0.f;
+                    for (int e = 0; e < 8; ++e) hi[e] = mid[e] = lo[e] = 0.f;
                 }
                 *chunk_at(to, r, cc) = pack8(hi);
-                *chunk_at(to + BOX, r, cc) = pack8(lo);
+                *chunk_at(to + BOX, r, cc) = pack8(mid);
+                *chunk_at(to + 2 * BOX, r, cc) = pack8(lo);
             }
             if (len < Q) {
                 wait.on(&sh.k_loaded[i & 1], (i >> 1) & 1);
@@ -276,8 +280,8 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
             tc::fence_after_sync();
             wait.on(&sh.k_loaded[i & 1], (i >> 1) & 1);
             const char* kb = kt + (i & 1) * (KP / 64) * BOX;
-            const char* wb = ws + (i & 1) * 2 * BOX;
-            product<true, true, Q / 16, 2 * VT>(tm + 128 * (i & 1), kb, wb, false);  // both parts: 64 columns each
+            const char* wb = ws + (i & 1) * 3 * BOX;
+            product<true, true, Q / 16, 3 * VT>(tm + 192 * (i & 1), kb, wb, false);  // all parts: 64 columns each
             tc::commit(&sh.made[i & 1]);
         };
         if (issuer) {
@@ -294,7 +298,10 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
             __syncwarp();
             for (int i = 0; i < count; ++i) {
                 if (one) {
-                    bulk_store_read();  // the image of the step before has left shared memory: the next may take its place
+                    if (i > 0) {  // the image of the step before has left shared memory: the next may take its place
+                        bulk_store_read();
+                        mbar_arrive(&sh.img_free);
+                    }
                     if (i + 2 < count) {  // k of this step, once its product has been made
                         wait.on(&sh.made[i & 1], (i >> 1) & 1);
                         load_k(i + 2);
@@ -304,7 +311,7 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
                 __syncthreads();  // operand i + 1 and image i are there
                 if (one) {
                     if (i + 1 < count) multiply(i + 1);
-                    bulk_store(images + (((long long)chunk(i) * a.H + h) * g.tiles + tile) * planes * (KP * 128), img + (i & 1) * 2 * KP * 128,
+                    bulk_store(images + (((long long)chunk(i) * a.H + h) * g.tiles + tile) * planes * (KP * 128), img,
                                planes * (KP * 128));
                     if (i + 3 < count) load_v(i + 3);
                 }
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
             for (int i = 0; i < count; ++i) {
                 if (i + 1 < count) scale(i + 1, ssm_chunk(s, chunk(i + 1)).len);
                 // the image of the state in front of (behind) this chunk: row k, 16 columns
-                char* to = img + (i & 1) * 2 * KP * 128;
+                if (i > 0) wait.on(&sh.img_free, (i - 1) & 1);
                 if (k < KP) {
 #pragma unroll
                     for (int cc = 0; cc < 2; ++cc) {
@@ -335,8 +342,8 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
                             hi[e] = __bfloat162float(__float2bfloat16_rn(st[8 * cc + e]));
                             lo[e] = st[8 * cc + e] - hi[e];
                         }
-                        *chunk_at(to, k, c0 / 8 + cc) = pack8(hi);
-                        if (planes == 2) *chunk_at(to + KP * 128, k, c0 / 8 + cc) = pack8(lo);
+                        *chunk_at(img, k, c0 / 8 + cc) = pack8(hi);
+                        if (planes == 2) *chunk_at(img + KP * 128, k, c0 / 8 + cc) = pack8(lo);
                     }
                 }
                 float decay2 = 1.f;
@@ -349,13 +356,13 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
                 __syncthreads();
                 wait.on(&sh.made[i & 1], (i >> 1) & 1);
                 tc::fence_after_sync();
-                const unsigned from = tm + ((unsigned)(32 * (w & 3)) << 16) + 128 * (i & 1) + c0;
+                const unsigned from = tm + ((unsigned)(32 * (w & 3)) << 16) + 192 * (i & 1) + c0;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    float hi[8], lo[8];
-                    tmem_ld8x2(from + 8 * q, from + VT + 8 * q, hi, lo);
+                    float hi[8], mid[8], lo[8];
+                    tmem_ld8x3(from + 8 * q, from + VT + 8 * q, from + 2 * VT + 8 * q, hi, mid, lo);
 #pragma unroll
-                    for (int v = 0; v < 8; ++v) st[8 * q + v] = fmaf(decay, st[8 * q + v], hi[v] + lo[v]);
+                    for (int v = 0; v < 8; ++v) st[8 * q + v] = fmaf(decay, st[8 * q + v], hi[v] + (mid[v] + lo[v]));
                 }
                 decay = decay1, decay1 = decay2;
             }
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(WALK_THREADS + 32, 1) ssm_walk_kernel(const Tc
 #pragma unroll
             for (int v = 0; v < 16; ++v) st[v] = __int_as_float(0x7fc00000);
         }
-        if (w == 0) tc::tmem_free(tm, 256);
+        if (w == 0) tc::tmem_free(tm, 512);
     }
     if (end && k < a.K)
 #pragma unroll
@@ -656,7 +663,8 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
     const int per = (rep + g.splits - 1) / g.splits, h0 = hq * rep + blockIdx.z * per, h1 = min((hq + 1) * rep, h0 + per);
     if (h0 >= h1) return;                  // (the launch leaves no share empty)
     if (tid == 0) {
-        for (unsigned long long* b : {&qk_loaded, &loaded, &inner, &pv, &outer}) tc::mbar_init(b);
+        for (unsigned long long* b : {&qk_loaded, &inner, &pv, &outer}) tc::mbar_init(b);
+        mbar_init_n(&loaded, 4);
         tc::mbar_init_fence();
     }
     if (w == 0) tc::tmem_alloc(&slot, 512);
@@ -665,13 +673,17 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
     tc::fence_after_sync();
     // do v^T, then P^T do over it; q h and k G; dq and dk
     const unsigned tm = slot, tD = tm, tU = tm + 128, tG = tm + 192, tQ = tm + 256, tK = tm + 256 + KP;
-    auto load = [&](int h, int tile) {  // one thread
-        tc::mbar_expect_tx(&loaded, 2 * BOX + 4 * KP * 128);
-        tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &loaded);
-        tma_load_3d(dy, &dmap, tile * VT, h, (int)ch.tok, &loaded);
+    // a head's tiles, one each by four threads: a copy takes its thread some 500 cycles
+    auto load = [&](int h, int tile) {
+        const int part = w == 8 ? 0 : w == 12 ? 1 : w == 13 ? 2 : w == 14 ? 3 : -1;
+        if (part < 0 || lane) return;
+        const unsigned bytes = part < 2 ? BOX : 2 * KP * 128;
+        tc::mbar_expect_tx(&loaded, bytes);
         const long long at = (((long long)c * a.H + h) * g.tiles + tile) * 2 * (KP * 128);
-        bulk_load(ht, g.state + at, 2 * KP * 128, &loaded);
-        bulk_load(gt, g.grad + at, 2 * KP * 128, &loaded);
+        if (part == 0) tma_load_3d(vt, &vmap, tile * VT, h, (int)ch.tok, &loaded);
+        else if (part == 1) tma_load_3d(dy, &dmap, tile * VT, h, (int)ch.tok, &loaded);
+        else if (part == 2) bulk_load(ht, g.state + at, bytes, &loaded);
+        else bulk_load(gt, g.grad + at, bytes, &loaded);
     };
     if (tid == ISSUER) {
         tc::mbar_expect_tx(&qk_loaded, 2 * (KP / 64) * BOX);
@@ -680,8 +692,9 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             tma_load_3d(qt + b * BOX, &qmap, 64 * b, hq, (int)ch.tok, &qk_loaded);
             tma_load_3d(kt + b * BOX, &kmap, 64 * b, hq, (int)ch.tok, &qk_loaded);
         }
-        load(h0, 0);
     }
+    load(h0, 0);
+    __syncwarp();
     Token next;
     if (tid < Q) next.ask(s, c, h0, tid), next.ask_gt(s, ch, h0, tid);
     Waits wait;
@@ -845,6 +858,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             if (tid == ISSUER) {
                 tc::fence_after_sync();
                 products<false, false, VT / 16, KP>(tQ, dy, ht, tK, vt, gt, step > 0);
+                products<false, false, VT / 16, KP>(tQ, dy, ht + KP * 128, tK, vt, gt + KP * 128, true);
                 tc::commit(&outer);
             }
             const int v0 = tile * VT;
@@ -860,73 +874,81 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
             tc::fence_after_sync();
             tc::fence_async_smem();
             __syncthreads();  // the tiles, and P behind dv, may be written again
-            if (tid == ISSUER) {
-                if (tile + 1 < g.tiles) load(h, tile + 1);
-                else if (h + 1 < h1) load(h + 1, 0);
-            }
-            if (tile + 1 == g.tiles) {  // the head's scalars: thread t of the first 128 has token t, of block b
+            if (tile + 1 < g.tiles) load(h, tile + 1);
+            else if (h + 1 < h1) load(h + 1, 0);
+            __syncwarp();
+            if (tile + 1 == g.tiles && tid < Q) {  // the head's scalars, by the first four warps: thread t has token t, of block b
                 const int t = tid, b = w;
-                float ta = 0.f, tb = 0.f, late = 0.f, own = 0.f, direct = 0.f, dt = 0.f;
-                if (tid < Q) {
-                    dt = x.dt[t];
-                    ta = x.eL[t] * ((sums.A[0][t] + sums.A[1][t]) + (sums.A[2][t] + sums.A[3][t]));
-                    own = x.wq[t] * ((sums.B[0][t] + sums.B[1][t]) + (sums.B[2][t] + sums.B[3][t]));
-                    tb = dt * own;
-                    direct = sums.col[b][t];
-                    for (int k = b + 1; k < 4; ++k) {
-                        const float y = sums.col[k][t];
-                        direct += y;
-                        late = fmaf(y, dt, late);
-                        const float total = warp_add(y * dt);
-                        if (lane == 0) sums.cross[k][b] = total;
-                    }
-                    const float at = warp_add(ta), bt = warp_add(tb);
-                    if (lane == 0) sums.at[b] = at, sums.bt[b] = bt;
+                float late = 0.f;
+                const float dt = x.dt[t];
+                const float ta = x.eL[t] * ((sums.A[0][t] + sums.A[1][t]) + (sums.A[2][t] + sums.A[3][t]));
+                const float own = x.wq[t] * ((sums.B[0][t] + sums.B[1][t]) + (sums.B[2][t] + sums.B[3][t])), tb = dt * own;
+                float direct = sums.col[b][t];
+                for (int k = b + 1; k < 4; ++k) {
+                    const float y = sums.col[k][t];
+                    direct += y;
+                    late = fmaf(y, dt, late);
+                    const float total = warp_add(y * dt);
+                    if (lane == 0) sums.cross[k][b] = total;
                 }
-                __syncthreads();
-                if (tid < Q) {
-                    float suf = ta, pre = late + tb;
-                    for (int k = 0; k < b; ++k) suf += sums.row[k][t];
+                const float at = warp_add(ta), bt = warp_add(tb);
+                if (lane == 0) sums.at[b] = at, sums.bt[b] = bt;
+                sync_group(1, Q);
+                float suf = ta, pre = late + tb;
+                for (int k = 0; k < b; ++k) suf += sums.row[k][t];
 #pragma unroll
-                    for (int d = 1; d < 32; d *= 2) {
-                        const float y = __shfl_down_sync(0xffffffffu, suf, d), u = __shfl_up_sync(0xffffffffu, pre, d);
-                        if (lane + d < 32) suf += y;
-                        if (lane >= d) pre += u;
-                    }
-                    pre = __shfl_up_sync(0xffffffffu, pre, 1);
-                    float dlf = sums.z[t] + suf + (lane ? pre : 0.f), hG = 0.f;
-                    for (int k = b + 1; k < 4; ++k) dlf += sums.at[k];
-                    for (int k = 0; k < b; ++k) dlf += sums.bt[k];
-                    for (int k = b + 1; k < 4; ++k)
-                        for (int i = 0; i < b; ++i) dlf += sums.cross[k][i];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) hG += sums.dot[k];
-                    dlf = fmaf(x.eL[Q - 1], hG, dlf);
-                    float ddt = direct + own - gh * dlf;
-                    float pg = 0.f, pb = 0.f;
-                    if (wait.bad) ddt = dlf = __int_as_float(0x7fc00000);
-                    if (t < ch.len) {
-                        const long long at = (ch.tok + t) * a.H + h;
-                        ddt *= ssm_ddt(u, (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0);
-                        st1(a.dgt, at, ddt, a.gt_dtype);
-                        pg = -dt * dlf, pb = ddt;
-                    }
-                    pg = warp_add(pg), pb = warp_add(pb);
-                    if (lane == 0) sums.pg[b] = pg, sums.pb[b] = pb;
+                for (int d = 1; d < 32; d *= 2) {
+                    const float y = __shfl_down_sync(0xffffffffu, suf, d), z = __shfl_up_sync(0xffffffffu, pre, d);
+                    if (lane + d < 32) suf += y;
+                    if (lane >= d) pre += z;
                 }
-                __syncthreads();
+                pre = __shfl_up_sync(0xffffffffu, pre, 1);
+                float dlf = sums.z[t] + suf + (lane ? pre : 0.f), hG = 0.f;
+                for (int k = b + 1; k < 4; ++k) dlf += sums.at[k];
+                for (int k = 0; k < b; ++k) dlf += sums.bt[k];
+                for (int k = b + 1; k < 4; ++k)
+                    for (int i = 0; i < b; ++i) dlf += sums.cross[k][i];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) hG += sums.dot[k];
+                dlf = fmaf(x.eL[Q - 1], hG, dlf);
+                float ddt = direct + own - gh * dlf;
+                float pg = 0.f, pb = 0.f;
+                if (wait.bad) ddt = dlf = __int_as_float(0x7fc00000);
+                if (t < ch.len) {
+                    ddt *= ssm_ddt(u, (a.flags & PALIMPSA_SSM_SOFTPLUS) != 0);
+                    st1(a.dgt, (ch.tok + t) * a.H + h, ddt, a.gt_dtype);
+                    pg = -dt * dlf, pb = ddt;
+                }
+                pg = warp_add(pg), pb = warp_add(pb);
+                if (lane == 0) sums.pg[b] = pg, sums.pb[b] = pb;
+                sync_group(1, Q);  // and the scalars may be written again; the sums are behind the next step's barrier
                 if (tid == 0) {
                     const long long n = (long long)s.chunks * a.H, at = (long long)c * a.H + h;
                     s.part[at] = sums.pg[0] + sums.pg[1] + sums.pg[2] + sums.pg[3];
                     s.part[n + at] = sums.pb[0] + sums.pb[1] + sums.pb[2] + sums.pb[3];
                     s.part[2 * n + at] = sums.diag[0] + sums.diag[1] + sums.diag[2] + sums.diag[3];
                 }
-                __syncthreads();  // the scalars and the sums may be written again
+                __syncwarp();
             }
         }
     }
     // dq += dS k, dk += dS^T q
-    if (cb <= rw) st_block(P, r, cb, dS);
+    // in two parts, once for all heads: the second where v and do have been
+    zero_tile(vt, 2 * BOX, tid, THREADS);
+    __syncthreads();
+    if (cb <= rw) {
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += 8) {
+            float hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                hi[e] = __bfloat162float(__float2bfloat16_rn(dS[i0 + e]));
+                lo[e] = dS[i0 + e] - hi[e];
+            }
+            *chunk_at(P + (cb >> 1) * BOX, r, (cb & 1) * 4 + i0 / 8) = pack8(hi);
+            *chunk_at(vt + (cb >> 1) * BOX, r, (cb & 1) * 4 + i0 / 8) = pack8(lo);
+        }
+    }
     tc::fence_async_smem();
     tc::fence_before_sync();
     __syncthreads();
@@ -934,6 +956,8 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
         tc::fence_after_sync();
         product<false, true, Q / 16, KP>(tQ, P, kt, true);
         product<true, true, Q / 16, KP>(tK, P, qt, true);
+        product<false, true, Q / 16, KP>(tQ, vt, kt, true);
+        product<true, true, Q / 16, KP>(tK, vt, qt, true);
         tc::commit(&outer);
     }
     wait.on(&outer, step & 1);
