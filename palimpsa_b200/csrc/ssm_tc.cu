@@ -11,9 +11,13 @@
 // operand (contraction along the columns) and as MN-major one (contraction along the tokens).  States cross memory as such images
 // too ([KP rows of d_k][64 columns of d_v], bfloat16, two parts hi + lo that give 16 bits), and are fetched by plain bulk copies.
 //
-// Roundings to bfloat16 (products are exact, sums float32 in TMEM): P, dS, e^L do and w dt v as operands of outputs in bfloat16,
-// once, 2^-9 rms of a term; hi of the state where o is made from it.  What ends in float32 -- the states, and q h and k G for the
-// gradients of dt, g and D -- takes both parts of its operand (2^-17), and S and do v^T of the decays' gradients stay float32.
+// Roundings to bfloat16 (products are exact, sums float32 in TMEM): P, e^L do and w dt v as operands of outputs in bfloat16, once,
+// 2^-9 rms of a term; hi of the state where o is made from it.  The states take w dt v in three parts (24 bits); dS, and the states as
+// operands of dq and dk, go in two parts (2^-17), as do those of q h and k G for the gradients of dt, g and D, while S and do v^T of the
+// decays' gradients stay float32.  Errors: o 0.0018, dq 0.0022 (bfloat16's own rounding: 0.0017), states 1e-7, dg and dgt_bias 1e-6 to 3e-6.
+//
+// What bounds them (24 heads of 128x64 on one q/k head, 16384 tokens, 148 SMs; floors by bytes 23, 23 and 54 us): walk 80 us, two waves
+// of 16 steps of 2.5 us, each CUDA-core work of 512 threads and one barrier; outputs 54; gradients 227, a chain of 16000 cycles a head.
 //
 // Rows of a tile behind a sequence's end are other tokens' or fill; they are zeroed in shared memory, so that whatever they hold
 // never meets a zero weight as NaN.  Every wait is bounded: one that gives up sets g_ssm_status, and what its CTA writes last (states, outputs,
@@ -163,8 +167,8 @@ struct Waits {
 // w v is taken in three parts (24 bits), so that the states are those of float32: 1e-7, with two parts 2e-6.
 // Steps are pipelined: while the product of step i runs, the operand of step i+1 is scaled and the image of the state in front of
 // step i is written out, so that a step costs its CUDA-core work and one barrier.  Everything a step writes has two buffers; k and
-// v are asked for one and two steps ahead.  (One step after the other, two CTAs an SM: 66 us for 192 walks of 16 steps, 69 for 64 of
-// 24; so: see ssm_tc_fwd.)
+// v are asked for one and two steps ahead.  (192 walks of 16 steps, 64 of 24, two parts: one step after the other, two CTAs an SM, 66
+// and 69 us; overlapped, one of the working threads issuing, 97 and 68; so 69 and 43, and with three parts 80 and 51.)
 constexpr int WALK_THREADS = 512;  // and a warp that issues products and copies (3000 cycles a step, if a warp does it beside its share);
                                    // thread: row k = tid % 128 of the state, 16 columns of d_v by tid / 128
 struct WalkShared {
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(Q * out_groups<KP>(), 3 - out_groups<KP>()) ss
 
 // ---- gradients ------------------------------------------------------------------------------------------------------------------------
 // 16 warps: warp w has rows 32 (w % 4) .. and the block of 32 columns w / 4 (16 columns of a tile of d_v).  (8 warps with two blocks
-// each: 19 500 cycles a head, a quarter of them in the one warp with the longest blocks.)
+// each: 246 us, 19 500 cycles a head, a quarter of them in the one warp with the longest blocks; so 227.)
 constexpr int THREADS = 512;
 constexpr int ISSUER = 384;  // issues products and loads: of warp 12, whose block lies above the diagonal, so that it has time
 struct GradSums {            // of a head, over its tiles
