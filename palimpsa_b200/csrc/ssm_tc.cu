@@ -633,7 +633,7 @@ struct GradSums {            // of a head, over its tiles
     float col[4][Q];         // sum over the rows of block w of P_ij (do_i.v_j): M_ij / dt_j
     float z[Q];              // sum_{i>=t>j} M_ij inside t's own block
     float A[4][Q], B[4][Q];  // do_i.(h q_i), v_j.(G k_j), by quarters of d_v
-    float dot[16], diag[4];  // <h, G>; do_i.v_i
+    float dot[5], diag[4];   // <h, G>; do_i.v_i
     float cross[4][4], at[4], bt[4], pg[4], pb[4];
 };
 template <int KP>
@@ -804,6 +804,20 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 }
                 xreduce<32, 32>(t, lane);
                 put(sums.col[rw][32 * cb + xreduce_index<32, 32>(lane)], t[0]);
+            } else if (w != ISSUER / 32) {  // <h, G>, by the five other warps that have no block: 4, 8, 9, 13, 14
+                const int part = w == 4 ? 0 : w < 12 ? w - 7 : w - 10;
+                float d = 0.f;
+                for (int i = 32 * part + lane; i < KP * 8; i += 160) {
+                    float p[8], q[8], u8[8], v[8];
+                    unpack8(reinterpret_cast<const uint4*>(ht)[i], p);
+                    unpack8(reinterpret_cast<const uint4*>(ht + KP * 128)[i], q);
+                    unpack8(reinterpret_cast<const uint4*>(gt)[i], u8);
+                    unpack8(reinterpret_cast<const uint4*>(gt + KP * 128)[i], v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) d = fmaf(p[e] + q[e], u8[e] + v[e], d);
+                }
+                d = warp_add(d);
+                if (lane == 0) put(sums.dot[part], d);
             }
             tc::fence_async_smem();
             tc::fence_before_sync();
@@ -812,20 +826,6 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 tc::fence_after_sync();
                 product<true, true, Q / 16, VT>(tD, P, dy, false);
                 tc::commit(&pv);
-            }
-            {   // <h, G>
-                float d = 0.f;
-                for (int i = tid; i < KP * 8; i += THREADS) {
-                    float p[8], q[8], u[8], v[8];
-                    unpack8(reinterpret_cast<const uint4*>(ht)[i], p);
-                    unpack8(reinterpret_cast<const uint4*>(ht + KP * 128)[i], q);
-                    unpack8(reinterpret_cast<const uint4*>(gt)[i], u);
-                    unpack8(reinterpret_cast<const uint4*>(gt + KP * 128)[i], v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) d = fmaf(p[e] + q[e], u[e] + v[e], d);
-                }
-                d = warp_add(d);
-                if (lane == 0) put(sums.dot[w], d);
             }
             wait.on(&pv, step & 1);
             tc::fence_after_sync();
@@ -913,7 +913,7 @@ __global__ void __launch_bounds__(THREADS, 1) ssm_grad_tc_kernel(const TcArgs g,
                 for (int k = b + 1; k < 4; ++k)
                     for (int i = 0; i < b; ++i) dlf += sums.cross[k][i];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) hG += sums.dot[k];
+                for (int k = 0; k < 5; ++k) hG += sums.dot[k];
                 dlf = fmaf(x.eL[Q - 1], hG, dlf);
                 float ddt = direct + own - gh * dlf;
                 float pg = 0.f, pb = 0.f;
