@@ -60,12 +60,11 @@ __device__ __forceinline__ void seq_span(const int* cu, long long seq_len, long 
     }
 }
 
-// N consecutive values of an io type: one or two 16-byte accesses where `vec` says that the address allows it.
+// N = 4 or 8 consecutive values of an io type: in wide accesses where `vec` says that the address allows it.
 template <int DT, int N>
 __device__ __forceinline__ void ld_n(const void* base, long long idx, int live, bool vec, float (&x)[N]) {
-    if (N >= 4 && vec) {
-        if constexpr (N < 4) {
-        } else if constexpr (DT == PALIMPSA_F32) {
+    if (vec) {
+        if constexpr (DT == PALIMPSA_F32) {
 #pragma unroll
             for (int i = 0; i < N / 4; ++i) {
                 const float4 y = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + idx)[i];
